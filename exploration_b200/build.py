@@ -36,6 +36,12 @@ SOURCES = [
     "attention/gated_tc_bwd.cu",
     "sparse/sparse_read.cu",
     "sparse/block_scores_tc.cu",
+    "paged/paged_append.cu",
+    "paged/paged_entry.cu",
+    "paged/paged_simt.cu",
+    "paged/paged_combine.cu",
+    "beam/beam_select.cu",
+    "beam/beam_reorder.cu",
     "gemm/gemm_tc.cu",
     "comm/symm_heap.cu",
     "comm/grad_reduce.cu",

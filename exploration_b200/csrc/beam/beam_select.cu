@@ -1,0 +1,383 @@
+// Beam search's selection: the best `beams` continuations of a group of beams.
+//
+// Beam w at cumulative score c_w offers token t at c_w + (x_wt - lse_w) with
+// lse_w = log sum_t exp(x_wt); an ended beam offers only (eos, c_w). Inside a
+// beam candidates are ordered by logit, then by token; across beams by score,
+// then by beam: rounding of the sum never reorders a beam's tokens, so each
+// beam's best `beams` logits are all that the final choice needs. A beam
+// whose lse is not finite (nothing left unmasked, or a NaN) offers -inf only.
+//
+// Bound by one read of the logits (and by latency below a few MB). A warp holds
+// 1,024 logits in registers and takes its maximum, sum and best K from there:
+// per-lane bests, then K rounds of warp maximum / lowest index
+// (redux.sync on order-preserving integers). Up to 1,024 tokens one CTA a group
+// with a warp a beam does all in one launch. Longer rows are cut into chunks of
+// 8,192, one CTA each, whose sums and best K a second, overlapped launch joins:
+// sums of chunks in fp64, so lse does not depend on the cut beyond its rounding.
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <climits>
+
+#include "../common/util.cuh"
+
+namespace eb {
+namespace {
+
+constexpr int kPerLane = 32;
+constexpr int kWarpTokens = 32 * kPerLane;
+constexpr int kChunkWarps = 8;
+constexpr int kChunk = kChunkWarps * kWarpTokens;
+constexpr int kMaxBeams = 32;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct SelectArgs {
+  const void* logits;        // [rows, vocab], dense
+  const float* scores;       // [rows]
+  const bool* finished;
+  float* scores_out;
+  int64_t* parents;
+  int64_t* tokens;
+  bool* finished_out;
+  float* part_ms;            // [rows, chunks, 2]
+  float* part_x;             // [rows, chunks, beams]
+  int* part_t;
+  int beams, vocab, chunks, keep, eos;   // keep = min(beams, vocab)
+};
+
+// Order-preserving map of floats to unsigned integers.
+EB_DEVICE uint32_t ordered(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+EB_DEVICE float unordered(uint32_t u) {
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+
+// A lane's logits: kPerLane / VE vectors, vector j at index (j * 32 + lane) * VE of
+// the warp's span. Absent ones are -inf. `begin` may lie before the row (alignment).
+template <typename T>
+struct LaneLogits {
+  static constexpr int VE = 16 / sizeof(T);
+  float x[kPerLane];
+  int64_t begin;   // token index of the warp's span
+
+  EB_DEVICE int token(int i, int lane) const {
+    return static_cast<int>(begin) + ((i / VE) * 32 + lane) * VE + i % VE;
+  }
+
+  EB_DEVICE void load(const T* row, int64_t from, int vocab, int lane) {
+    begin = from;
+#pragma unroll
+    for (int j = 0; j < kPerLane / VE; ++j) {
+      const int64_t t = from + (j * 32 + lane) * VE;
+      if (t >= 0 && t + VE <= vocab) {
+        const uint4 u = *reinterpret_cast<const uint4*>(row + t);
+        const T* h = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) x[j * VE + i] = load_f<T>(h + i) + 0.f;   // -0 ties with 0
+      } else {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) 
+          x[j * VE + i] = t + i >= 0 && t + i < vocab ? load_f<T>(row + t + i) + 0.f : kNegInf;
+      }
+    }
+  }
+
+  // Maximum and sum of 2^((x - max) log2 e) over the warp.
+  EB_DEVICE void sum(float& m, float& s) const {
+    m = kNegInf;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) m = fmaxf(m, x[i]);
+    m = warp_max(m);
+    const float ref = finite_or_zero(m);
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) s += ex2((x[i] - ref) * kLog2e);
+    s = warp_sum(s);
+  }
+
+  // Calls take(round, value, token) in every lane for the best `count` logits in order.
+  template <typename F>
+  EB_DEVICE void best(int count, int vocab, int lane, F take) const {
+    uint32_t used = 0;
+    uint32_t key = 0;
+    int slot = 0;
+    auto rescan = [&]() {
+      key = 0;   // below every float's key
+      slot = -1;
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) {
+        const int t = token(i, lane);
+        const uint32_t k = ordered(x[i]);
+        if (!(used >> i & 1) && t >= 0 && t < vocab && (slot < 0 || k > key)) {
+          key = k;
+          slot = i;
+        }
+      }
+    };
+    rescan();
+    for (int round = 0; round < count; ++round) {
+      const uint32_t top = __reduce_max_sync(0xffffffffu, slot < 0 ? 0u : key);
+      const int mine = slot >= 0 && key == top ? token(slot, lane) : INT_MAX;
+      const int first = __reduce_min_sync(0xffffffffu, mine);
+      take(round, unordered(top), first);
+      if (mine == first && first != INT_MAX) {
+        used |= 1u << slot;
+        rescan();
+      }
+    }
+  }
+};
+
+// Token index of the first 16-byte boundary at or before `row`'s chunk start.
+template <typename T>
+EB_DEVICE int64_t aligned_start(const T* row) {
+  constexpr int VE = 16 / sizeof(T);
+  const int ahead = static_cast<int>((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % VE);
+  return -ahead;
+}
+
+// One warp: the best `beams` of the beams' sorted candidate lists total[w][i], token[w][i] (shared memory).
+EB_DEVICE void choose(const SelectArgs& p, int group, int lane, const float (*total)[kMaxBeams],
+                      const int (*token)[kMaxBeams]) {
+  int at = 0;
+  const bool ended = lane < p.beams && p.finished[group * p.beams + lane];
+  for (int round = 0; round < p.beams; ++round) {
+    const bool live = lane < p.beams && at < p.keep;
+    const uint32_t key = live ? ordered(total[lane][at] + 0.f) : 0u;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, key);
+    const int winner = __ffs(__ballot_sync(0xffffffffu, live && key == top)) - 1;
+    if (lane == winner) {
+      const int64_t out = static_cast<int64_t>(group) * p.beams + round;
+      p.scores_out[out] = total[lane][at];
+      p.parents[out] = lane;
+      p.tokens[out] = token[lane][at];
+      p.finished_out[out] = ended || token[lane][at] == p.eos;
+      ++at;
+    }
+  }
+}
+
+// Candidate i of a beam with logit x: its total score.
+EB_DEVICE void offer(const SelectArgs& p, int row, float lse, int i, float x, int t, float& total, int& token) {
+  const float base = p.scores[row];
+  if (p.finished[row]) {
+    total = i == 0 ? base : kNegInf;
+    token = p.eos;
+  } else {
+    const float sum = __fadd_rn(base, __fsub_rn(x, lse));
+    total = isfinite(lse) && sum == sum ? sum : kNegInf;
+    token = t;
+  }
+}
+
+// Up to kWarpTokens tokens: one CTA a group, one warp a beam.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+beam_select_small_kernel(SelectArgs p) {
+  __shared__ float total[kMaxBeams][kMaxBeams];
+  __shared__ int token[kMaxBeams][kMaxBeams];
+  const int group = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = group * p.beams + warp;
+  {
+    const T* logits = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.vocab;
+    LaneLogits<T> x;
+    x.load(logits, aligned_start(logits), p.vocab, lane);
+    float m, s;
+    x.sum(m, s);
+    const float lse = m + logf(s);
+    x.best(p.keep, p.vocab, lane, [&](int i, float value, int t) {
+      if (lane == 0) offer(p, row, lse, i, value, t, total[warp][i], token[warp][i]);
+    });
+  }
+  __syncthreads();
+  if (warp == 0) choose(p, group, lane, total, token);
+}
+
+// Longer rows, first launch: sums and best K of one chunk.
+template <typename T>
+__global__ void __launch_bounds__(kChunkWarps * 32)
+beam_select_chunk_kernel(SelectArgs p) {
+  __shared__ float sm_m[kChunkWarps], sm_s[kChunkWarps];
+  __shared__ float sm_x[kChunkWarps][kMaxBeams];
+  __shared__ int sm_t[kChunkWarps][kMaxBeams];
+  const int chunk = blockIdx.x, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const T* logits = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.vocab;
+  {
+    LaneLogits<T> x;
+    x.load(logits, aligned_start(logits) + static_cast<int64_t>(chunk) * kChunk + warp * kWarpTokens, p.vocab, lane);
+    float m, s;
+    x.sum(m, s);
+    if (lane == 0) {
+      sm_m[warp] = m;
+      sm_s[warp] = s;
+    }
+    x.best(p.keep, p.vocab, lane, [&](int i, float value, int t) {
+      if (lane == 0) {
+        sm_x[warp][i] = value;
+        sm_t[warp][i] = t;
+      }
+    });
+  }
+  __syncthreads();
+  if (warp != 0) return;
+  const int64_t part = static_cast<int64_t>(row) * p.chunks + chunk;
+  float m = lane < kChunkWarps ? sm_m[lane] : kNegInf;
+  const float top = warp_max(m), ref = finite_or_zero(top);
+  const float s = warp_sum(lane < kChunkWarps ? sm_s[lane] * ex2((m - ref) * kLog2e) : 0.f);
+  if (lane == 0) {
+    p.part_ms[part * 2] = top;
+    p.part_ms[part * 2 + 1] = s;
+  }
+  int at = 0;
+  for (int round = 0; round < p.keep; ++round) {
+    const bool live = lane < kChunkWarps && at < p.keep && sm_t[lane][at] != INT_MAX;
+    const uint32_t key = live ? ordered(sm_x[lane][at]) : 0u;
+    const uint32_t best = __reduce_max_sync(0xffffffffu, key);
+    // Lower warps hold lower tokens: the first of equal logits is the lowest token.
+    const int winner = __ffs(__ballot_sync(0xffffffffu, live && key == best)) - 1;
+    if (winner < 0) {
+      if (lane == 0) {
+        p.part_x[part * p.keep + round] = kNegInf;
+        p.part_t[part * p.keep + round] = INT_MAX;
+      }
+    } else if (lane == winner) {
+      p.part_x[part * p.keep + round] = sm_x[lane][at];
+      p.part_t[part * p.keep + round] = sm_t[lane][at];
+      ++at;
+    }
+  }
+}
+
+// Second launch: one CTA a group, one warp a beam joins its chunks, then the choice.
+__global__ void __launch_bounds__(1024)
+beam_select_join_kernel(SelectArgs p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ float total[kMaxBeams][kMaxBeams];
+  __shared__ int token[kMaxBeams][kMaxBeams];
+  const int group = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = group * p.beams + warp;
+  const int64_t base = static_cast<int64_t>(row) * p.chunks;
+  float m = kNegInf;
+  for (int c = lane; c < p.chunks; c += 32) m = fmaxf(m, p.part_ms[(base + c) * 2]);
+  m = warp_max(m);
+  const float ref = finite_or_zero(m);
+  double sum = 0.0;
+  for (int c = lane; c < p.chunks; c += 32) {
+    const float2 ms = *reinterpret_cast<const float2*>(p.part_ms + (base + c) * 2);
+    sum += static_cast<double>(ms.y) * exp(static_cast<double>(ms.x) - ref);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float lse = static_cast<float>(static_cast<double>(m) + log(sum));
+  // K rounds over the chunks' sorted lists: chunk c belongs to lane c % 32.
+  uint32_t key = 0;
+  int mine = INT_MAX;
+  // A lane with several chunks rescans their lists for its best entry after (last value, last token).
+  uint32_t last_key = 0xffffffffu;
+  int last_t = -1;
+  auto rescan = [&]() {
+    key = 0;
+    mine = INT_MAX;
+    for (int c = lane; c < p.chunks; c += 32) {
+      for (int i = 0; i < p.keep; ++i) {
+        const int t = p.part_t[(base + c) * p.keep + i];
+        if (t == INT_MAX) break;
+        const uint32_t k = ordered(p.part_x[(base + c) * p.keep + i]);
+        if (k > last_key || (k == last_key && t <= last_t)) continue;   // taken before
+        if (mine == INT_MAX || k > key || (k == key && t < mine)) {
+          key = k;
+          mine = t;
+        }
+        break;
+      }
+    }
+  };
+  rescan();
+  for (int round = 0; round < p.keep; ++round) {
+    const uint32_t top = __reduce_max_sync(0xffffffffu, mine == INT_MAX ? 0u : key);
+    const int cand = mine != INT_MAX && key == top ? mine : INT_MAX;
+    const int first = __reduce_min_sync(0xffffffffu, cand);
+    if (lane == 0) offer(p, row, lse, round, unordered(top), first, total[warp][round], token[warp][round]);
+    if (cand == first && first != INT_MAX) {
+      last_key = key;
+      last_t = mine;
+      rescan();
+    }
+  }
+  __syncthreads();
+  if (warp == 0) choose(p, group, lane, total, token);
+}
+
+template <typename T>
+void launch(SelectArgs& args, int groups, const at::TensorOptions& f32, cudaStream_t stream) {
+  if (args.vocab + 16 / static_cast<int>(sizeof(T)) - 1 <= kWarpTokens) {
+    beam_select_small_kernel<T><<<groups, 32 * args.beams, 0, stream>>>(args);
+    EB_CUDA_CHECK(cudaGetLastError());
+    count_launch(1);
+    return;
+  }
+  const int64_t rows = static_cast<int64_t>(groups) * args.beams;
+  // One chunk more than the vocabulary needs when the row starts inside a vector.
+  args.chunks = cdiv(args.vocab + 16 / static_cast<int>(sizeof(T)) - 1, kChunk);
+  at::Tensor ms = at::empty({rows, args.chunks, 2}, f32);
+  at::Tensor x = at::empty({rows, args.chunks, args.keep}, f32);
+  at::Tensor t = at::empty({rows, args.chunks, args.keep}, f32.dtype(at::kInt));
+  args.part_ms = ms.data_ptr<float>();
+  args.part_x = x.data_ptr<float>();
+  args.part_t = t.data_ptr<int>();
+  beam_select_chunk_kernel<T><<<dim3(args.chunks, rows), kChunkWarps * 32, 0, stream>>>(args);
+  EB_CUDA_CHECK(cudaGetLastError());
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(groups);
+  config.blockDim = dim3(32 * args.beams);
+  config.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  EB_CUDA_CHECK(cudaLaunchKernelEx(&config, beam_select_join_kernel, args));
+  count_launch(2);
+}
+
+}  // namespace
+
+std::vector<at::Tensor> beam_select(const at::Tensor& logits, const at::Tensor& scores, const at::Tensor& finished,
+                                    int64_t eos) {
+  c10::cuda::CUDAGuard guard(logits.device());
+  const int64_t groups = logits.size(0), beams = logits.size(1), vocab = logits.size(2);
+  TORCH_CHECK(beams <= kMaxBeams, "beam_select: at most ", kMaxBeams, " beams");
+  TORCH_CHECK(groups * beams < 65536 && vocab < (1LL << 30), "beam_select: too many rows or tokens");
+  at::Tensor scores_out = at::empty_like(scores);
+  at::Tensor parents = at::empty({groups, beams}, scores.options().dtype(at::kLong));
+  at::Tensor tokens = at::empty_like(parents);
+  at::Tensor finished_out = at::empty_like(finished);
+  if (groups * beams > 0) {
+    SelectArgs args{};
+    args.logits = logits.data_ptr();
+    args.scores = scores.data_ptr<float>();
+    args.finished = finished.data_ptr<bool>();
+    args.scores_out = scores_out.data_ptr<float>();
+    args.parents = parents.data_ptr<int64_t>();
+    args.tokens = tokens.data_ptr<int64_t>();
+    args.finished_out = finished_out.data_ptr<bool>();
+    args.beams = beams;
+    args.vocab = vocab;
+    args.keep = std::min(beams, vocab);
+    args.eos = eos;
+    auto stream = at::cuda::getCurrentCUDAStream();
+    switch (logits.scalar_type()) {
+      case at::kFloat: launch<float>(args, groups, scores.options(), stream); break;
+      case at::kHalf: launch<__half>(args, groups, scores.options(), stream); break;
+      case at::kBFloat16: launch<__nv_bfloat16>(args, groups, scores.options(), stream); break;
+      default: TORCH_CHECK(false, "beam_select: fp32, fp16 or bf16 logits");
+    }
+  }
+  return {scores_out, parents, tokens, finished_out};
+}
+
+}  // namespace eb

@@ -100,6 +100,16 @@ std::vector<at::Tensor> block_scores_topk_tc(const at::Tensor& q, const at::Tens
 std::vector<at::Tensor> sparse_pop(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                    const at::Tensor& pos, const at::Tensor& ids, const at::Tensor& scores,
                                    const at::Tensor& log_zr, int64_t block, int64_t offset);
+at::Tensor paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cos,
+                        const at::Tensor& sin, at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& tables,
+                        const at::Tensor& positions);
+std::string paged_attention_path(const at::Tensor& q, const at::Tensor& k_cache);
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                           const at::Tensor& tables, const at::Tensor& positions);
+std::vector<at::Tensor> beam_select(const at::Tensor& logits, const at::Tensor& scores, const at::Tensor& finished,
+                                    int64_t eos);
+std::vector<at::Tensor> beam_reorder(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& tables,
+                                     const at::Tensor& spare, const at::Tensor& parents, const at::Tensor& lengths);
 }  // namespace eb
 
 namespace {
@@ -173,6 +183,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("block_scores_tc_supported", &eb::block_scores_tc_supported);
   m.def("block_scores_topk_tc", &eb::block_scores_topk_tc,
         "tcgen05 exact block scores with log Z_R and a radix-select top-k per row");
+  m.def("paged_append", &eb::paged_append, "rotate queries and keys, write keys and values into their pages");
+  m.def("paged_attention_path", &eb::paged_attention_path);
+  m.def("paged_attention", &eb::paged_attention, "attention of new tokens over a paged cache");
+  m.def("beam_select", &eb::beam_select, "best continuations of every group of beams");
+  m.def("beam_reorder", &eb::beam_reorder, "new tables and copies of partly filled pages after a selection");
   m.def("launch_count", &eb::launch_count, "kernels launched by this extension so far");
   m.def("device_errors", &device_errors, "read and clear (site, cta) of the last bounded-wait timeout");
 }

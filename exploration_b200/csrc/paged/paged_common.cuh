@@ -1,0 +1,193 @@
+// Shared pieces of the paged-cache attention kernels: the argument block, the
+// split of the work over the CTAs of a launch, and the partial results that
+// the combine kernel joins.
+//
+// A cache is a pool of pages [pages, kv_heads, page, dim]; `tables[b, j]`
+// names the pool page with the keys of positions [j * page, (j + 1) * page) of
+// sequence b. Query heads h * group .. h * group + group - 1 share key head h,
+// so the rows of one (sequence, key head) are row r = token * group + g. A
+// group larger than a kernel's row tile is divided into several items of the
+// same key head.
+//
+// Work split. An entry is a (sequence, row tile); its key limit is one more
+// than the largest position among its rows, so nothing but `positions` (on
+// the device) says how long a sequence is: one captured launch serves every
+// later step. The key tiles of all (entry, key head) items form one list, cut
+// into equal runs, one a CTA: sequences of very different lengths and a few
+// rows over a long cache both fill the GPU. An item inside one run is written
+// out by its CTA; an item that is cut leaves unnormalised partial sums (at most
+// two a CTA: its first and its last item), which the combine kernel joins in
+// key order, so results do not depend on the order in which CTAs finish.
+#pragma once
+
+#include "../common/util.cuh"
+
+namespace eb {
+namespace paged {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxEntries = 2048;   // entries whose tile counts fit the CTA's shared prefix table
+
+struct Args {
+  const void* q;          // [batch, tokens, heads, dim], dense
+  const void* k;          // [pages, kv_heads, page, dim], dense
+  const void* v;
+  const int* tables;      // [batch, width]
+  const int* positions;   // [batch, tokens], -1: no row
+  void* out;              // like q
+  float* part_o;          // [2 * CTAs, row_tile, dim] partial sums of 2^(a - m) v
+  float* part_ml;         // [2 * CTAs, row_tile, 2]: m (base 2), sum of 2^(a - m)
+  int* cum;               // [entries + 1] prefix of key tiles, written by CTA 0 for the combine kernel
+  int batch, tokens, heads, kv_heads, dim;
+  int group;              // query heads of an item
+  int item_heads;         // items of an entry: kv_heads, or a multiple when an item takes part of a head's group
+  int head_div;           // item_heads / kv_heads
+  int pages, page, page_shift, width;
+  int row_tile;           // rows of a row tile (a whole number of tokens)
+  int tile_tokens;        // its tokens
+  int row_tiles;          // row tiles of a sequence
+  int key_tile;           // keys of a tile
+  int flat;               // 1: equal runs of the tile list; 0: one item a CTA (too many entries for the table)
+  int min_run;            // fewest tiles of a run
+  float scale_log2;       // log2(e) / sqrt(dim)
+};
+
+struct Segment {
+  int entry, head;        // the item
+  int batch, token0;      // its sequence and first token
+  int begin, end;         // key tiles
+  int limit;              // keys of the item
+  int slot;               // partial slot, -1: the whole item (written out)
+};
+
+// Largest position of an entry's rows plus one, inside the table; 0 when it has no row.
+EB_DEVICE int entry_limit(const Args& p, int entry) {
+  const int b = entry / p.row_tiles, t0 = (entry - b * p.row_tiles) * p.tile_tokens;
+  const int n = min(p.tile_tokens, p.tokens - t0);
+  const int* pos = p.positions + static_cast<int64_t>(b) * p.tokens + t0;
+  int top = -1;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) top = max(top, pos[i]);
+  return static_cast<int>(min(static_cast<int64_t>(top) + 1, static_cast<int64_t>(p.width) * p.page));
+}
+
+EB_DEVICE int entry_limit_warp(const Args& p, int entry, int lane) {
+  const int b = entry / p.row_tiles, t0 = (entry - b * p.row_tiles) * p.tile_tokens;
+  const int n = min(p.tile_tokens, p.tokens - t0);
+  const int* pos = p.positions + static_cast<int64_t>(b) * p.tokens + t0;
+  int top = -1;
+  for (int i = lane; i < n; i += 32) top = max(top, pos[i]);
+  top = __reduce_max_sync(0xffffffffu, top);
+  return static_cast<int>(min(static_cast<int64_t>(top) + 1, static_cast<int64_t>(p.width) * p.page));
+}
+
+// Prefix of the entries' key tiles into cum[0 .. entries] (shared memory); all threads.
+EB_DEVICE void build_prefix(const Args& p, int* cum) {
+  const int entries = p.batch * p.row_tiles;
+  if (p.tile_tokens <= 16) {
+    for (int e = threadIdx.x; e < entries; e += blockDim.x)
+      cum[e + 1] = cdiv(entry_limit(p, e), p.key_tile);
+  } else {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int e = warp; e < entries; e += blockDim.x >> 5) {
+      const int n = entry_limit_warp(p, e, lane);
+      if (lane == 0) cum[e + 1] = cdiv(n, p.key_tile);
+    }
+  }
+  if (threadIdx.x == 0) cum[0] = 0;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int carry = 0;
+    for (int base = 0; base < entries; base += 32) {
+      const int i = base + threadIdx.x;
+      int x = i < entries ? cum[i + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (static_cast<int>(threadIdx.x) >= o) x += y;
+      }
+      x += carry;
+      if (i < entries) cum[i + 1] = x;
+      carry = __shfl_sync(0xffffffffu, x, 31);
+    }
+  }
+  __syncthreads();
+}
+
+// Tiles of one run.
+EB_DEVICE int64_t run_tiles(const Args& p, int total, int ctas) {
+  const int64_t all = static_cast<int64_t>(total) * p.item_heads;
+  const int64_t run = (all + ctas - 1) / ctas;
+  return run < p.min_run ? p.min_run : run;
+}
+
+// Walks the segments of one CTA's run. `cum` is unused when flat == 0.
+struct Walk {
+  int64_t at, end, first;
+  int entry_hint;
+
+  EB_DEVICE void start(const Args& p, const int* cum) {
+    if (p.flat) {
+      const int total = cum[p.batch * p.row_tiles];
+      const int64_t run = run_tiles(p, total, gridDim.x), all = static_cast<int64_t>(total) * p.item_heads;
+      at = static_cast<int64_t>(blockIdx.x) * run;
+      end = at + run < all ? at + run : all;
+    } else {
+      // Latest row tiles first: they hold the most keys of a causal chunk.
+      at = static_cast<int64_t>(p.batch) * p.row_tiles * p.item_heads - 1 - blockIdx.x;
+      end = at + 1;
+    }
+    first = at;
+    entry_hint = 0;
+  }
+
+  // The next segment, or false. Uniform over the threads that call it. In the
+  // one-item form the segment may be empty (begin == end, slot -1): the output is zero.
+  EB_DEVICE bool next(const Args& p, const int* cum, Segment& s) {
+    if (at >= end) return false;
+    int tiles;
+    if (p.flat) {
+      const int entries = p.batch * p.row_tiles;
+      int lo = entry_hint, hi = entries;
+      while (hi - lo > 1) {   // last entry whose items start at or before `at` (never an empty one)
+        const int mid = (lo + hi) >> 1;
+        if (static_cast<int64_t>(cum[mid]) * p.item_heads <= at) lo = mid;
+        else hi = mid;
+      }
+      s.entry = lo;
+      entry_hint = lo;
+      tiles = cum[lo + 1] - cum[lo];
+      const int64_t rel = at - static_cast<int64_t>(cum[lo]) * p.item_heads;
+      s.head = static_cast<int>(rel / tiles);
+      s.begin = static_cast<int>(rel - static_cast<int64_t>(s.head) * tiles);
+      s.end = static_cast<int>(min(static_cast<int64_t>(tiles), s.begin + (end - at)));
+      s.slot = s.begin == 0 && s.end == tiles ? -1 : 2 * blockIdx.x + (at == first ? 0 : 1);
+      at += s.end - s.begin;
+    } else {
+      s.entry = static_cast<int>(at / p.item_heads);
+      s.head = static_cast<int>(at - static_cast<int64_t>(s.entry) * p.item_heads);
+      s.slot = -1;
+      ++at;
+    }
+    s.batch = s.entry / p.row_tiles;
+    s.token0 = (s.entry - s.batch * p.row_tiles) * p.tile_tokens;
+    return true;
+  }
+};
+
+// Limit of a segment's item, and for the one-item form its tiles; every thread of a warp calls it.
+EB_DEVICE void finish_segment(const Args& p, Segment& s, int lane) {
+  s.limit = entry_limit_warp(p, s.entry, lane);
+  if (!p.flat) {
+    s.begin = 0;
+    s.end = cdiv(s.limit, p.key_tile);
+  }
+}
+
+}  // namespace paged
+
+// Joins the partial sums of cut items and zeroes the rows of empty entries (paged_combine.cu).
+template <typename T>
+void paged_combine_launch(const paged::Args& args, int ctas, cudaStream_t stream);
+
+}  // namespace eb

@@ -1,0 +1,70 @@
+// Host side of the paged-attention kernels: row tiles, split and workspace.
+#pragma once
+
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+
+#include <algorithm>
+
+#include "paged_common.cuh"
+
+namespace eb {
+namespace paged {
+
+// Row tiles of at most `most` rows: whole tokens of a group; a group that is
+// larger is divided into equal parts, each an item of its own.
+inline void set_rows(Args& args, int most, int key_tile) {
+  const int whole = args.heads / args.kv_heads;
+  int part = whole;
+  while (part > most || whole % part) --part;
+  args.group = part;
+  args.head_div = whole / part;
+  args.item_heads = args.kv_heads * args.head_div;
+  args.tile_tokens = std::min(args.tokens, std::max(1, most / part));
+  args.row_tile = args.tile_tokens * part;
+  args.row_tiles = cdiv(args.tokens, args.tile_tokens);
+  args.key_tile = key_tile;
+  args.min_run = 1;
+}
+
+// The split of one call: CTAs, and the workspace of the cut items. The
+// workspace comes from the stream-ordered caching allocator and is given back
+// when the call has been enqueued.
+struct Split {
+  int ctas = 0;
+  at::Tensor part_o, part_ml, cum;
+
+  Split(Args& args, int wanted, cudaStream_t) {
+    const int64_t entries = static_cast<int64_t>(args.batch) * args.row_tiles;
+    const int64_t items = entries * args.item_heads;
+    args.flat = entries <= kMaxEntries;
+    if (!args.flat) {
+      TORCH_CHECK(items < (1LL << 31), "paged_attention: too many rows");
+      ctas = static_cast<int>(items);
+      return;
+    }
+    const int64_t longest = cdiv64(static_cast<int64_t>(args.width) * args.page, args.key_tile);
+    ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(wanted, items * longest)));
+    auto f32 = at::TensorOptions().device(at::kCUDA, at::cuda::current_device()).dtype(at::kFloat);
+    part_o = at::empty({2LL * ctas, args.row_tile, args.dim}, f32);
+    part_ml = at::empty({2LL * ctas, args.row_tile, 2}, f32);
+    cum = at::empty({entries + 1}, f32.dtype(at::kInt));
+    args.part_o = part_o.data_ptr<float>();
+    args.part_ml = part_ml.data_ptr<float>();
+    args.cum = cum.data_ptr<int>();
+  }
+
+  static int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+  template <typename T>
+  void combine(const Args& args, cudaStream_t stream) const {
+    if (args.flat) paged_combine_launch<T>(args, ctas, stream);
+  }
+};
+
+}  // namespace paged
+
+template <typename T>
+void paged_simt_launch(paged::Args& args, int sms, cudaStream_t stream);
+
+}  // namespace eb
