@@ -10,8 +10,20 @@ namespace eb {
 
 using paged::Args;
 
+namespace {
+
+// Few rows of a key head: the kernel bound by the read of the cache.
+bool rows_path(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache) {
+  const int64_t dim = q.size(3);
+  auto aligned = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; };
+  return q.scalar_type() != at::kFloat && (dim == 64 || dim == 128) && aligned(q) && aligned(k_cache) &&
+         aligned(v_cache);
+}
+
+}  // namespace
+
 std::string paged_attention_path(const at::Tensor& q, const at::Tensor& k_cache) {
-  return "cuda_core";
+  return rows_path(q, k_cache, k_cache) ? "rows" : "cuda_core";
 }
 
 at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
@@ -20,7 +32,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   at::Tensor out = at::empty_like(q);
   if (q.numel() == 0) return out;
   TORCH_CHECK(q.size(0) * q.size(1) * q.size(2) < (1LL << 31), "paged_attention: too many rows");
-  TORCH_CHECK(tables.size(1) * k_cache.size(2) < (1LL << 31), "paged_attention: tables are too wide");
+  TORCH_CHECK(tables.size(1) * k_cache.size(2) < (1LL << 30), "paged_attention: tables are too wide");
   if (tables.size(1) == 0 || k_cache.size(0) == 0) return out.zero_();
   Args args{};
   args.q = q.data_ptr();
@@ -41,6 +53,11 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   args.scale_log2 = static_cast<float>(paged::kLog2e / std::sqrt(static_cast<double>(args.dim)));
   auto stream = at::cuda::getCurrentCUDAStream();
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  if (rows_path(q, k_cache, v_cache)) {
+    if (q.scalar_type() == at::kHalf) paged_rows_launch<__half>(args, sms, stream);
+    else paged_rows_launch<__nv_bfloat16>(args, sms, stream);
+    return out;
+  }
   switch (q.scalar_type()) {
     case at::kFloat: paged_simt_launch<float>(args, sms, stream); break;
     case at::kHalf: paged_simt_launch<__half>(args, sms, stream); break;

@@ -6,10 +6,33 @@
 
 #include <algorithm>
 
+#include "../common/tma.cuh"
 #include "paged_common.cuh"
 
 namespace eb {
 namespace paged {
+
+// The pool [pages * kv_heads, page, dim] of a 16-bit type for TMA loads of one
+// plane's `rows` x 64 boxes (at most a page), 128-byte swizzle. Planes past the
+// pool read as zero.
+inline CUtensorMap make_pool_map(const Args& args, const void* base, bool half, int rows) {
+  bind_primary_context();
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(base) % 16 == 0, "paged_attention: pools must be 16-byte aligned");
+  const int64_t planes = static_cast<int64_t>(args.pages) * args.kv_heads;
+  TORCH_CHECK(planes < (1LL << 31) - 1, "paged_attention: too many pages");
+  CUtensorMap map;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(args.dim), static_cast<cuuint64_t>(args.page),
+                        static_cast<cuuint64_t>(planes)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(args.dim) * 2, static_cast<cuuint64_t>(args.page) * args.dim * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(std::min(args.page, rows)), 1};
+  cuuint32_t unit[3] = {1, 1, 1};
+  CUresult res = tensor_map_encoder()(&map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                      3, const_cast<void*>(base), dims, strides, box, unit,
+                                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(res == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with ", static_cast<int>(res));
+  return map;
+}
 
 // Row tiles of at most `most` rows: whole tokens of a group; a group that is
 // larger is divided into equal parts, each an item of its own.
@@ -66,5 +89,7 @@ struct Split {
 
 template <typename T>
 void paged_simt_launch(paged::Args& args, int sms, cudaStream_t stream);
+template <typename T>
+void paged_rows_launch(paged::Args& args, int sms, cudaStream_t stream);
 
 }  // namespace eb
