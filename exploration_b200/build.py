@@ -40,6 +40,7 @@ SOURCES = [
     "paged/paged_entry.cu",
     "paged/paged_simt.cu",
     "paged/paged_rows.cu",
+    "paged/paged_chunk_tc.cu",
     "paged/paged_combine.cu",
     "beam/beam_select.cu",
     "beam/beam_reorder.cu",

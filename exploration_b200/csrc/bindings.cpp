@@ -103,7 +103,7 @@ std::vector<at::Tensor> sparse_pop(const at::Tensor& q, const at::Tensor& k, con
 at::Tensor paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cos,
                         const at::Tensor& sin, at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& tables,
                         const at::Tensor& positions);
-std::string paged_attention_path(const at::Tensor& q, const at::Tensor& k_cache);
+std::string paged_attention_path(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache);
 at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
                            const at::Tensor& tables, const at::Tensor& positions);
 std::vector<at::Tensor> beam_select(const at::Tensor& logits, const at::Tensor& scores, const at::Tensor& finished,

@@ -1,0 +1,499 @@
+// Attention of a chunk of new tokens over a paged cache on the 5th-generation
+// tensor cores (16-bit types, head dim 64 or 128, more than 16 rows of a key head).
+//
+// out[r] = sum_{i <= pos_r} softmax(q_r . k_i / sqrt(D)) v_i with the running
+// maximum and sum of one pass (base 2, fp32). Rows are packed token by token,
+// the query heads of a key head side by side, so small chunks with shared heads
+// still fill the 128 rows of an MMA.
+//
+// One CTA walks its run of (item, 128-key tile) pairs. Warp roles (384 threads):
+//   warp 0       producer: Q once an item, K and V tiles (a TMA box a page,
+//                128-byte swizzle) into two rings
+//   warp 1       MMA issuer: S = Q K^T into TMEM, O += P V with P read from TMEM
+//   warp 2       TMEM owner (512 columns)
+//   warps 4-7    softmax warpgroup 0, one thread a row (TMEM lane)
+//   warps 8-11   softmax warpgroup 1
+// Items of more than 128 rows give each warpgroup its own 128 rows of every key
+// tile; smaller ones give both the same rows and alternate key tiles, joined
+// through TMEM at the item's end. Either way the issuer alternates between the
+// warpgroups: while one exponentiates its scores, the other's products run.
+//
+// P (16 bit) overwrites its scores' TMEM columns. A running maximum is kept
+// until it grows by more than 2^8 (then O is rescaled in TMEM): S of step k + 2
+// is issued after P V of step k, so a finished S means a finished O.
+//
+// TMEM columns: S/P of warpgroup w at [128 w, 128 w + 128), O at [256 + D w, ...).
+//
+// Keys past an item's limit are masked, and their rows of the last V tile are
+// cleared in shared memory: a page's unwritten rows may hold anything.
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+
+#include <climits>
+
+#include "../common/sm100.cuh"
+#include "../common/tma.cuh"
+#include "paged_common.cuh"
+#include "paged_launch.h"
+#include "paged_mma.cuh"
+
+namespace eb {
+namespace {
+
+using namespace paged;
+using namespace sm100;
+
+constexpr int kM = 128;               // rows of an MMA
+constexpr int kTile = 128;            // keys of a tile
+constexpr int kBox = 128 * 64;        // elements of a 64-wide half of a 128-row operand
+constexpr int kThreads = 384;
+constexpr int kTmemCols = 512;
+constexpr float kRescale = 8.f;       // log2 units
+
+template <int D>
+struct alignas(1024) ChunkSmem {
+  static constexpr int kStages = D == 64 ? 4 : 2;   // of each ring
+  uint16_t q[2][kM * D];
+  uint16_t k[kStages][kTile * D];
+  uint16_t v[kStages][kTile * D];
+  uint64_t q_full, q_empty;
+  uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+  uint64_t s_full[2], p_full[2], o_full[2], join;
+  uint32_t tmem_base;
+  int abort;
+  float ml[kM][2];
+  int cum[kMaxEntries + 1];
+};
+
+// Positions in the two rings and of the barriers' phases, carried across items.
+struct Ring {
+  int stage = 0, phase = 0;
+  EB_DEVICE void next(int stages) {
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// Keeps the compiler from using TMEM loads before the wait that precedes this.
+template <int N>
+EB_DEVICE void hold(uint32_t (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                   const __grid_constant__ CUtensorMap tv, Args p, ErrorSlot* err) {
+  extern __shared__ __align__(1024) uint8_t raw_smem[];
+  ChunkSmem<D>& sm = *reinterpret_cast<ChunkSmem<D>*>(
+      (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+  constexpr int kStages = ChunkSmem<D>::kStages;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort = &sm.abort;
+  if (threadIdx.x == 0) {
+    mbar_init(&sm.q_full, 1);
+    mbar_init(&sm.q_empty, 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&sm.k_full[s], 1);
+      mbar_init(&sm.k_empty[s], 1);
+      mbar_init(&sm.v_full[s], 1);
+      mbar_init(&sm.v_empty[s], 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&sm.s_full[w], 1);
+      mbar_init(&sm.p_full[w], 128);
+      mbar_init(&sm.o_full[w], 1);
+    }
+    mbar_init(&sm.join, 256);
+    sm.abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 2) tmem_alloc(&sm.tmem_base, kTmemCols);
+  if (p.flat) build_prefix(p, sm.cum);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = sm.tmem_base;
+  Walk walk;
+  walk.start(p, sm.cum);
+  publish_run<T>(p, sm.cum, walk);
+  Segment s;
+  const int half_tokens = kM / p.group;         // tokens of one warpgroup's rows
+  const int half_rows = half_tokens * p.group;
+  // Both warpgroups have rows of their own when the item holds more tokens than one takes.
+  auto split_rows = [&](const Segment& seg) { return p.tokens - seg.token0 > half_tokens; };
+
+  if (warp == 0) {
+    const int box = min(p.page, kTile), boxes_tile = kTile / box;
+    if (lane == 0) {
+      prefetch_tensormap(&tq);
+      prefetch_tensormap(&tk);
+      prefetch_tensormap(&tv);
+    }
+    Ring ring;            // K and V advance together
+    int q_loads = 0, tiles_issued = 0;
+    bool ok = true;
+    while (ok && walk.next(p, sm.cum, s)) {
+      finish_segment(p, s, lane);
+      if (s.begin == s.end) continue;
+      const int kv_head = s.head / p.head_div;
+      if (q_loads > 0 && !__all_sync(0xffffffffu, mbar_wait(&sm.q_empty, (q_loads - 1) & 1, abort, err, kSiteQFull)))
+        break;
+      const int halves = split_rows(s) ? 2 : 1;
+      if (lane == 0) {
+        mbar_expect_tx(&sm.q_full, halves * half_rows * D * 2);
+        for (int w = 0; w < halves; ++w)
+#pragma unroll
+          for (int h = 0; h < D / 64; ++h)
+            tma_load_4d(&sm.q[w][h * kBox], &tq, &sm.q_full, h * 64, s.head * p.group, s.token0 + w * half_tokens,
+                        s.batch);
+      }
+      ++q_loads;
+      const int* table = p.tables + static_cast<int64_t>(s.batch) * p.width;
+      const int last_page = (s.limit - 1) >> p.page_shift;
+      auto entry = [&](int page) { return page <= last_page ? table[page] : -1; };
+      int base = (s.begin * kTile) >> p.page_shift;
+      int ids = entry(base + lane), ahead = entry(base + 32 + lane);
+      for (int tile = s.begin; tile < s.end; ++tile) {
+        const int key0 = tile * kTile;
+        const int boxes = min(boxes_tile, cdiv(s.limit - key0, box));
+        // Plane of box i in lane i (at most eight boxes a tile). An entry outside
+        // the pool reads as zeros (out of the map's bounds), never foreign memory.
+        const int first_page = key0 >> p.page_shift;
+        if (first_page - base >= 32) {
+          base += 32;
+          ids = ahead;
+          ahead = entry(base + 32 + lane);
+        }
+        const int want = ((key0 + min(lane, boxes - 1) * box) >> p.page_shift) - base;
+        const int id_low = __shfl_sync(0xffffffffu, ids, want & 31), id_high = __shfl_sync(0xffffffffu, ahead, want & 31);
+        const int id = want < 32 ? id_low : id_high;
+        const int plane = id >= 0 && id < p.pages ? id * p.kv_heads + kv_head : p.pages * p.kv_heads;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          uint64_t* full = part == 0 ? &sm.k_full[ring.stage] : &sm.v_full[ring.stage];
+          uint64_t* empty = part == 0 ? &sm.k_empty[ring.stage] : &sm.v_empty[ring.stage];
+          uint16_t* dst = part == 0 ? sm.k[ring.stage] : sm.v[ring.stage];
+          const CUtensorMap* map = part == 0 ? &tk : &tv;
+          if (tiles_issued >= kStages &&
+              !__all_sync(0xffffffffu, mbar_wait(empty, ring.phase ^ 1, abort, err, kSiteKvEmpty))) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) mbar_expect_tx(full, boxes * box * D * 2);
+          __syncwarp();
+          if (lane < boxes) {
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h)
+              tma_load_3d(dst + h * kBox + lane * box * 64, map, full, h * 64, (key0 + lane * box) & (p.page - 1),
+                          plane);
+          }
+        }
+        if (!ok) break;
+        ++tiles_issued;
+        ring.next(kStages);
+      }
+    }
+    if (*abort && lane == 0) {   // let issued copies land before the CTA exits
+      for (int j = max(0, tiles_issued - kStages); j < tiles_issued; ++j) {
+        mbar_wait(&sm.k_full[j % kStages], (j / kStages) & 1, abort, nullptr, kSiteDrain);
+        mbar_wait(&sm.v_full[j % kStages], (j / kStages) & 1, abort, nullptr, kSiteDrain);
+      }
+      if (q_loads > 0) mbar_wait(&sm.q_full, (q_loads - 1) & 1, abort, nullptr, kSiteDrain);
+    }
+  } else if (warp == 1) {
+    constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+    const uint32_t id_s = idesc_16(kBf16, kM, kTile, false, false);
+    const uint32_t id_pv = idesc_16(kBf16, kM, D, false, true);
+    Ring kr, vr;
+    int segments = 0;
+    uint32_t p_phase = 0;   // bit w: parity of warpgroup w's next weights
+    bool ok = true;
+    while (ok && walk.next(p, sm.cum, s)) {
+      finish_segment(p, s, lane);
+      if (s.begin == s.end) continue;
+      const bool dual = split_rows(s);
+      const int tiles = s.end - s.begin, steps = dual ? 2 * tiles : tiles;
+      if (!__all_sync(0xffffffffu, mbar_wait(&sm.q_full, segments & 1, abort, err, kSiteQFull))) break;
+      ++segments;
+      // Step i belongs to warpgroup i & 1; with rows of their own both take each tile.
+      auto issue_s = [&](int i) -> bool {
+        const int w = i & 1;
+        if (!dual || w == 0) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&sm.k_full[kr.stage], kr.phase, abort, err, kSiteKvFull))) return false;
+        }
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t q_addr = smem_u32(sm.q[dual ? w : 0]), k_addr = smem_u32(sm.k[kr.stage]);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk / 4) * kBox * 2 + (kk % 4) * 32;
+            mma_ss(tmem + w * 128, smem_desc_sw128(q_addr + off, 16, 1024), smem_desc_sw128(k_addr + off, 16, 1024),
+                   id_s, kk > 0);
+          }
+          tc_commit(&sm.s_full[w]);
+          if (!dual || w == 1) tc_commit(&sm.k_empty[kr.stage]);
+          if (i == steps - 1) tc_commit(&sm.q_empty);
+        }
+        __syncwarp();
+        if (!dual || w == 1) kr.next(kStages);
+        return true;
+      };
+      ok = issue_s(0) && (steps == 1 || issue_s(1));
+      for (int i = 0; ok && i < steps; ++i) {
+        const int w = i & 1, tile = s.begin + (dual ? i >> 1 : i);
+        if (!dual || w == 0) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&sm.v_full[vr.stage], vr.phase, abort, err, kSiteKvFull))) {
+            ok = false;
+            break;
+          }
+          const int valid = s.limit - tile * kTile;
+          if (valid < kTile) {   // rows past the limit: cleared once, before the first product that reads them
+            uint4* rows = reinterpret_cast<uint4*>(sm.v[vr.stage]);
+            for (int j = valid * 8 + lane; j < kTile * 8; j += 32)
+#pragma unroll
+              for (int h = 0; h < D / 64; ++h) rows[h * (kBox / 8) + j] = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(&sm.p_full[w], p_phase >> w & 1, abort, err, kSitePFull))) {
+          ok = false;
+          break;
+        }
+        p_phase ^= 1u << w;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t v_addr = smem_u32(sm.v[vr.stage]);
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk)
+            mma_ts(tmem + 256 + w * D, tmem + w * 128 + kk * 8, smem_desc_sw128(v_addr + kk * 2048, kBox * 2, 1024),
+                   id_pv, i > 1 || kk > 0);
+          if (!dual || w == 1) tc_commit(&sm.v_empty[vr.stage]);
+          if (i >= steps - 2) tc_commit(&sm.o_full[w]);
+        }
+        __syncwarp();
+        if (!dual || w == 1) vr.next(kStages);
+        if (i + 2 < steps) ok = issue_s(i + 2);
+      }
+    }
+  } else if (warp >= 4) {
+    const int w = (warp >> 2) - 1;                   // softmax warpgroup
+    const int row = (warp & 3) * 32 + lane;          // TMEM lane
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t s_addr = lane_addr + w * 128;
+    int steps_done = 0, segments = 0, joins = 0;
+    bool ok = true;
+    // Both warpgroups, bounded: TMEM accesses before it are ordered before those after it.
+    auto join = [&]() -> bool {
+      tc_fence_before();
+      mbar_arrive(&sm.join);
+      const bool met = __all_sync(0xffffffffu, mbar_wait(&sm.join, joins & 1, abort, err, kSiteODone));
+      ++joins;
+      tc_fence_after();
+      return met;
+    };
+    while (ok && walk.next(p, sm.cum, s)) {
+      finish_segment(p, s, lane);
+      const bool dual = split_rows(s);
+      const int first = dual ? w * half_tokens : 0;
+      const int token = s.token0 + first + row / p.group;
+      const bool present = row < half_rows && token < p.tokens;
+      const int64_t flat_token = static_cast<int64_t>(s.batch) * p.tokens + token;
+      const int pos = present ? p.positions[flat_token] : -1;
+      const int see = pos >= 0 ? pos : INT_MAX;      // absent rows need no mask: nothing of theirs is written
+      const int low = __reduce_min_sync(0xffffffffu, see);
+      float m = kNegInf, l = 0.f;
+      const int stride = dual ? 1 : 2;
+      int begun = 0;
+      for (int tile = s.begin + (dual ? 0 : w); tile < s.end; tile += stride, ++begun) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[w], steps_done & 1, abort, err, kSiteSFull))) {
+          ok = false;
+          break;
+        }
+        ++steps_done;
+        tc_fence_after();
+        float x[kTile];
+#pragma unroll
+        for (int c = 0; c < kTile; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(s_addr + c, r);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[c + i] = __uint_as_float(r[i]);
+        }
+        tc_wait_ld();
+#pragma unroll
+        for (int c = 0; c < kTile; ++c) asm volatile("" : "+f"(x[c]));   // no use before the wait
+        const int key0 = tile * kTile;
+        if (key0 + kTile - 1 > low || key0 + kTile > s.limit) {
+          const int last = min(see, s.limit - 1) - key0;
+#pragma unroll
+          for (int c = 0; c < kTile; ++c)
+            if (c > last) x[c] = kNegInf;
+        }
+        float top[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (int c = 4; c < kTile; c += 4)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], x[c + i]);
+        const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+        float alpha = 1.f;
+        if (peak > m + kRescale || m == kNegInf) {
+          alpha = ex2(m - finite_or_zero(peak));     // 0 at the first key
+          m = peak;
+        }
+        if (begun > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+          for (int c = 0; c < D; c += 16) {
+            uint32_t r[16];
+            tmem_ld16(lane_addr + 256 + w * D + c, r);
+            tc_wait_ld();
+            hold(r);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+            tmem_st16(lane_addr + 256 + w * D + c, r);
+          }
+        }
+        const float ref = finite_or_zero(m);
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kTile; c += 32) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float e0 = ex2(fmaf(x[c + 2 * i], p.scale_log2, -ref));
+            const float e1 = ex2(fmaf(x[c + 2 * i + 1], p.scale_log2, -ref));
+            sum[(2 * i) & 3] += e0;
+            sum[(2 * i + 1) & 3] += e1;
+            packed[i] = pack2<T>(e0, e1);   // weights rounded for the second product, their sum is not
+          }
+          tmem_st16(s_addr + c / 2, packed);
+        }
+        l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(&sm.p_full[w]);
+      }
+      if (!ok) break;
+      if (begun > 0) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&sm.o_full[w], segments & 1, abort, err, kSiteODone))) break;
+        ++segments;
+        tc_fence_after();
+      }
+      if (pos < 0) {   // a padding row: zero, no weight
+        m = kNegInf;
+        l = 0.f;
+      }
+      float other_m = kNegInf, other_l = 0.f;
+      if (!dual) {
+        // Warpgroup 1 leaves its statistics; warpgroup 0 reads both accumulators and writes.
+        if (w == 1) {
+          sm.ml[row][0] = begun > 0 ? m : kNegInf;
+          sm.ml[row][1] = begun > 0 ? l : 0.f;
+        }
+        if (!join()) break;
+        if (w == 0) {
+          other_m = sm.ml[row][0];
+          other_l = sm.ml[row][1];
+        }
+      }
+      if (dual || w == 0) {
+        const bool two = !dual && s.end - s.begin > 1;
+        const float best = fmaxf(m, other_m), ref = finite_or_zero(best);
+        float f0 = ex2(m - ref), f1 = ex2(other_m - ref);
+        const float total = f0 * l + f1 * other_l;
+        const bool write = present, whole = s.slot < 0;
+        if (whole) {
+          const float inv = total == 0.f ? 0.f : 1.f / total;
+          f0 *= inv;
+          f1 *= inv;
+        }
+        const int qhead = s.head * p.group + row % p.group;
+        T* dst = static_cast<T*>(p.out) + ((present ? flat_token : 0) * p.heads + qhead) * D;
+        const int64_t part = static_cast<int64_t>(s.slot) * p.row_tile + first * p.group + row;
+        if (!whole && write) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(best, total);
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          uint32_t r[32];
+          if (s.begin < s.end) {
+            tmem_ld32(lane_addr + 256 + w * D + c, r);
+            tc_wait_ld();
+            hold(r);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = pos >= 0 ? __uint_as_float(r[i]) * f0 : 0.f;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0.f;
+          }
+          if (two) {
+            tmem_ld32(lane_addr + 256 + D + c, r);
+            tc_wait_ld();
+            hold(r);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] += pos >= 0 ? __uint_as_float(r[i]) * f1 : 0.f;
+          }
+          if (write && whole) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              *reinterpret_cast<uint4*>(dst + c + i) =
+                  make_uint4(pack2<T>(o[i], o[i + 1]), pack2<T>(o[i + 2], o[i + 3]), pack2<T>(o[i + 4], o[i + 5]),
+                             pack2<T>(o[i + 6], o[i + 7]));
+          } else if (write) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(p.part_o + part * D + c + i) =
+                  make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+        }
+      }
+      tc_fence_before();
+      if (!dual && !join()) break;   // accumulators and statistics have been read
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <typename T, int D>
+void launch(Args& args, int sms, cudaStream_t stream) {
+  const Split split(args, sms, stream);
+  constexpr bool kHalf = std::is_same_v<T, __half>;
+  const CUtensorMap tq = make_query_map(args, kHalf, kM / args.group);
+  const CUtensorMap tk = make_pool_map(args, args.k, kHalf, kTile);
+  const CUtensorMap tv = make_pool_map(args, args.v, kHalf, kTile);
+  const size_t smem = sizeof(ChunkSmem<D>) + 1024;
+  auto kernel = paged_chunk_kernel<T, D>;
+  EB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kernel<<<split.ctas, kThreads, smem, stream>>>(tq, tk, tv, args, device_error_slot(at::cuda::current_device()));
+  EB_CUDA_CHECK(cudaGetLastError());
+  count_launch(1);
+  split.combine<T>(args, stream);
+}
+
+}  // namespace
+
+template <typename T>
+void paged_chunk_launch(Args& args, int sms, cudaStream_t stream) {
+  set_rows(args, kM, kTile);
+  // Two MMAs' rows an item when there are more than one MMA's.
+  const int half_tokens = kM / args.group;
+  args.tile_tokens = std::min(args.tokens, 2 * half_tokens);
+  args.row_tile = args.tile_tokens * args.group;
+  args.row_tiles = cdiv(args.tokens, args.tile_tokens);
+  if (args.dim == 64) return launch<T, 64>(args, sms, stream);
+  return launch<T, 128>(args, sms, stream);
+}
+
+template void paged_chunk_launch<__half>(Args&, int, cudaStream_t);
+template void paged_chunk_launch<__nv_bfloat16>(Args&, int, cudaStream_t);
+
+}  // namespace eb

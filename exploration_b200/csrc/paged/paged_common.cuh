@@ -17,7 +17,8 @@
 // rows over a long cache both fill the GPU. An item inside one run is written
 // out by its CTA; an item that is cut leaves unnormalised partial sums (at most
 // two a CTA: its first and its last item), which the combine kernel joins in
-// key order, so results do not depend on the order in which CTAs finish.
+// key order, so results do not depend on the order in which CTAs finish. Each
+// CTA notes where its run begins, so joining needs no search.
 #pragma once
 
 #include "../common/util.cuh"
@@ -37,7 +38,8 @@ struct Args {
   void* out;              // like q
   float* part_o;          // [2 * CTAs, row_tile, dim] partial sums of 2^(a - m) v
   float* part_ml;         // [2 * CTAs, row_tile, 2]: m (base 2), sum of 2^(a - m)
-  int* cum;               // [entries + 1] prefix of key tiles, written by CTA 0 for the combine kernel
+  int* cuts;              // [CTAs, 4]: entry, head, first tile and tiles of the item that a CTA's run begins in
+  int* run;               // [1] tiles of a run
   int batch, tokens, heads, kv_heads, dim;
   int group;              // query heads of an item
   int item_heads;         // items of an entry: kv_heads, or a multiple when an item takes part of a head's group
@@ -161,7 +163,7 @@ struct Walk {
       s.head = static_cast<int>(rel / tiles);
       s.begin = static_cast<int>(rel - static_cast<int64_t>(s.head) * tiles);
       s.end = static_cast<int>(min(static_cast<int64_t>(tiles), s.begin + (end - at)));
-      s.slot = s.begin == 0 && s.end == tiles ? -1 : 2 * blockIdx.x + (at == first ? 0 : 1);
+      s.slot = s.begin == 0 && s.end == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (at == first ? 0 : 1);
       at += s.end - s.begin;
     } else {
       s.entry = static_cast<int>(at / p.item_heads);
@@ -175,6 +177,28 @@ struct Walk {
   }
 };
 
+// What the combine kernel needs, and the rows of entries without any key. All threads, after walk.start().
+template <typename T>
+EB_DEVICE void publish_run(const Args& p, const int* cum, const Walk& walk) {
+  if (!p.flat) return;
+  if (threadIdx.x == 0) {
+    Walk probe = walk;
+    Segment s;
+    int4 cut = make_int4(0, 0, 0, 0);
+    if (probe.next(p, cum, s)) cut = make_int4(s.entry, s.head, s.begin, cum[s.entry + 1] - cum[s.entry]);
+    reinterpret_cast<int4*>(p.cuts)[blockIdx.x] = cut;
+    if (blockIdx.x == 0) *p.run = static_cast<int>(run_tiles(p, cum[p.batch * p.row_tiles], gridDim.x));
+  }
+  const int entries = p.batch * p.row_tiles;
+  for (int e = blockIdx.x; e < entries; e += gridDim.x) {
+    if (cum[e + 1] != cum[e]) continue;
+    const int b = e / p.row_tiles, t0 = (e - b * p.row_tiles) * p.tile_tokens;
+    const int64_t n = static_cast<int64_t>(min(p.tile_tokens, p.tokens - t0)) * p.heads * p.dim;
+    T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.tokens + t0) * p.heads * p.dim;
+    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) out[i] = cast_f<T>(0.f);
+  }
+}
+
 // Limit of a segment's item, and for the one-item form its tiles; every thread of a warp calls it.
 EB_DEVICE void finish_segment(const Args& p, Segment& s, int lane) {
   s.limit = entry_limit_warp(p, s.entry, lane);
@@ -186,7 +210,7 @@ EB_DEVICE void finish_segment(const Args& p, Segment& s, int lane) {
 
 }  // namespace paged
 
-// Joins the partial sums of cut items and zeroes the rows of empty entries (paged_combine.cu).
+// Joins the partial sums of cut items (paged_combine.cu).
 template <typename T>
 void paged_combine_launch(const paged::Args& args, int ctas, cudaStream_t stream);
 

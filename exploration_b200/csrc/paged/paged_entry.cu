@@ -12,18 +12,34 @@ using paged::Args;
 
 namespace {
 
-// Few rows of a key head: the kernel bound by the read of the cache.
-bool rows_path(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache) {
+enum class Path { kCudaCore, kRows, kChunk };
+
+// The kernel of a call. Tensor-core forms take 16-bit types of head dim 64 or
+// 128 (one or two 128-byte swizzle spans); up to 16 rows of a key head go to the
+// few-row kernel, which is bound by the read of the cache.
+Path choose(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache) {
   const int64_t dim = q.size(3);
   auto aligned = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; };
-  return q.scalar_type() != at::kFloat && (dim == 64 || dim == 128) && aligned(q) && aligned(k_cache) &&
-         aligned(v_cache);
+  if (q.scalar_type() == at::kFloat || (dim != 64 && dim != 128) || !aligned(q) || !aligned(k_cache) ||
+      !aligned(v_cache))
+    return Path::kCudaCore;
+  return q.size(1) * (q.size(2) / k_cache.size(1)) <= 16 ? Path::kRows : Path::kChunk;
+}
+
+template <typename T>
+void launch(Path path, Args& args, int sms, cudaStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    if (path == Path::kRows) return paged_rows_launch<T>(args, sms, stream);
+    if (path == Path::kChunk) return paged_chunk_launch<T>(args, sms, stream);
+  }
+  paged_simt_launch<T>(args, sms, stream);
 }
 
 }  // namespace
 
-std::string paged_attention_path(const at::Tensor& q, const at::Tensor& k_cache) {
-  return rows_path(q, k_cache, k_cache) ? "rows" : "cuda_core";
+std::string paged_attention_path(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache) {
+  const Path path = choose(q, k_cache, v_cache);
+  return path == Path::kRows ? "rows" : path == Path::kChunk ? "tcgen05" : "cuda_core";
 }
 
 at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
@@ -53,15 +69,11 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   args.scale_log2 = static_cast<float>(paged::kLog2e / std::sqrt(static_cast<double>(args.dim)));
   auto stream = at::cuda::getCurrentCUDAStream();
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  if (rows_path(q, k_cache, v_cache)) {
-    if (q.scalar_type() == at::kHalf) paged_rows_launch<__half>(args, sms, stream);
-    else paged_rows_launch<__nv_bfloat16>(args, sms, stream);
-    return out;
-  }
+  const Path path = choose(q, k_cache, v_cache);
   switch (q.scalar_type()) {
-    case at::kFloat: paged_simt_launch<float>(args, sms, stream); break;
-    case at::kHalf: paged_simt_launch<__half>(args, sms, stream); break;
-    case at::kBFloat16: paged_simt_launch<__nv_bfloat16>(args, sms, stream); break;
+    case at::kFloat: launch<float>(path, args, sms, stream); break;
+    case at::kHalf: launch<__half>(path, args, sms, stream); break;
+    case at::kBFloat16: launch<__nv_bfloat16>(path, args, sms, stream); break;
     default: TORCH_CHECK(false, "paged_attention: fp32, fp16 or bf16");
   }
   return out;

@@ -34,6 +34,27 @@ inline CUtensorMap make_pool_map(const Args& args, const void* base, bool half, 
   return map;
 }
 
+// The queries [batch, tokens, heads, dim] for TMA loads of one item's rows: `tokens`
+// tokens of a group's heads (token by token), 128-byte swizzle. Tokens past the
+// call's read as zero.
+inline CUtensorMap make_query_map(const Args& args, bool half, int tokens) {
+  bind_primary_context();
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(args.q) % 16 == 0, "paged_attention: queries must be 16-byte aligned");
+  CUtensorMap map;
+  const cuuint64_t row = static_cast<cuuint64_t>(args.dim) * 2;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(args.dim), static_cast<cuuint64_t>(args.heads),
+                        static_cast<cuuint64_t>(args.tokens), static_cast<cuuint64_t>(args.batch)};
+  cuuint64_t strides[3] = {row, row * args.heads, row * args.heads * args.tokens};
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(args.group), static_cast<cuuint32_t>(tokens), 1};
+  cuuint32_t unit[4] = {1, 1, 1, 1};
+  CUresult res = tensor_map_encoder()(&map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                      4, const_cast<void*>(args.q), dims, strides, box, unit,
+                                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(res == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with ", static_cast<int>(res));
+  return map;
+}
+
 // Row tiles of at most `most` rows: whole tokens of a group; a group that is
 // larger is divided into equal parts, each an item of its own.
 inline void set_rows(Args& args, int most, int key_tile) {
@@ -55,7 +76,7 @@ inline void set_rows(Args& args, int most, int key_tile) {
 // when the call has been enqueued.
 struct Split {
   int ctas = 0;
-  at::Tensor part_o, part_ml, cum;
+  at::Tensor part_o, part_ml, cuts;
 
   Split(Args& args, int wanted, cudaStream_t) {
     const int64_t entries = static_cast<int64_t>(args.batch) * args.row_tiles;
@@ -71,17 +92,18 @@ struct Split {
     auto f32 = at::TensorOptions().device(at::kCUDA, at::cuda::current_device()).dtype(at::kFloat);
     part_o = at::empty({2LL * ctas, args.row_tile, args.dim}, f32);
     part_ml = at::empty({2LL * ctas, args.row_tile, 2}, f32);
-    cum = at::empty({entries + 1}, f32.dtype(at::kInt));
+    cuts = at::empty({4LL * ctas + 1}, f32.dtype(at::kInt));
     args.part_o = part_o.data_ptr<float>();
     args.part_ml = part_ml.data_ptr<float>();
-    args.cum = cum.data_ptr<int>();
+    args.cuts = cuts.data_ptr<int>();
+    args.run = args.cuts + 4LL * ctas;
   }
 
   static int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
   template <typename T>
   void combine(const Args& args, cudaStream_t stream) const {
-    if (args.flat) paged_combine_launch<T>(args, ctas, stream);
+    if (args.flat && ctas > 1) paged_combine_launch<T>(args, ctas, stream);
   }
 };
 
@@ -91,5 +113,7 @@ template <typename T>
 void paged_simt_launch(paged::Args& args, int sms, cudaStream_t stream);
 template <typename T>
 void paged_rows_launch(paged::Args& args, int sms, cudaStream_t stream);
+template <typename T>
+void paged_chunk_launch(paged::Args& args, int sms, cudaStream_t stream);
 
 }  // namespace eb

@@ -1,4 +1,5 @@
-// Warp-level matrix instructions of the few-row kernel and 16-bit packing.
+// Warp-level matrix instructions of the few-row kernel, 16-bit packing and the
+// tcgen05 instruction descriptor of the chunk kernel.
 #pragma once
 
 #include <type_traits>
@@ -47,6 +48,14 @@ EB_DEVICE uint32_t pack2(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
   }
+}
+
+// Instruction descriptor of kind::f16 with both operands fp16 or both bf16, fp32 accumulation.
+EB_HOST_DEVICE uint32_t idesc_16(bool bf16, int m, int n, bool a_mn_major, bool b_mn_major) {
+  const uint32_t type = bf16 ? 1u : 0u;
+  return (1u << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(a_mn_major) << 15) |
+         (static_cast<uint32_t>(b_mn_major) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
 }
 
 }  // namespace paged

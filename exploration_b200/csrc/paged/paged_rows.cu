@@ -80,10 +80,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   if (p.flat) build_prefix(p, sm.cum);
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (p.flat && blockIdx.x == 0)
-    for (int i = threadIdx.x; i <= p.batch * p.row_tiles; i += blockDim.x) p.cum[i] = sm.cum[i];
   Walk walk;
   walk.start(p, sm.cum);
+  publish_run<T>(p, sm.cum, walk);
   Segment s;
 
   if (warp == kConsumers) {

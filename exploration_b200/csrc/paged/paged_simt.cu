@@ -68,13 +68,10 @@ paged_simt_kernel(Args p) {
   const int grp = lane / LK, d0 = (lane % LK) * VE;
   const int valid = p.dim - d0;                   // elements of this lane's vector that exist
   const bool vec = (p.dim & 3) == 0;
-  if (p.flat) {
-    build_prefix(p, cum);
-    if (blockIdx.x == 0)
-      for (int i = threadIdx.x; i <= p.batch * p.row_tiles; i += blockDim.x) p.cum[i] = cum[i];
-  }
+  if (p.flat) build_prefix(p, cum);
   Walk walk;
   walk.start(p, cum);
+  publish_run<T>(p, cum, walk);
   Segment s;
   const T* q = static_cast<const T*>(p.q);
   const T* kc = static_cast<const T*>(p.k);

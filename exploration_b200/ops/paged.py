@@ -109,7 +109,7 @@ def paged_attention(q, k_cache, v_cache, tables, positions):
         ext = _native.native(q)
         out = ext.paged_attention(q.contiguous(), k_cache, v_cache, tables.contiguous(), _int32(positions))
         record("paged_attention", dtype=str(q.dtype), head_dim=q.shape[3], page=k_cache.shape[2],
-               path=ext.paged_attention_path(q, k_cache))
+               path=ext.paged_attention_path(q, k_cache, v_cache))
         return out
     return attention_reference(q, k_cache, v_cache, tables, positions)
 
