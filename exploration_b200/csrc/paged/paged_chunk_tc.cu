@@ -127,6 +127,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   // Both warpgroups have rows of their own when the item holds more tokens than one takes.
   auto split_rows = [&](const Segment& seg) { return p.tokens - seg.token0 > half_tokens; };
 
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == 0) {
     const int box = min(p.page, kTile), boxes_tile = kTile / box;
     if (lane == 0) {
@@ -281,7 +283,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         if (i + 2 < steps) ok = issue_s(i + 2);
       }
     }
-  } else if (warp >= 4) {
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int w = (warp >> 2) - 1;                   // softmax warpgroup
     const int row = (warp & 3) * 32 + lane;          // TMEM lane
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -337,9 +341,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         }
         float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int c = 4; c < kTile; c += 4)
+        for (int c = 4; c < kTile - 4; c += 8)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], x[c + i]);
+          for (int i = 0; i < 4; ++i) top[i] = max3(top[i], x[c + i], x[c + 4 + i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], x[kTile - 4 + i]);
         const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
         float alpha = 1.f;
         if (peak > m + kRescale || m == kNegInf) {
@@ -359,21 +365,23 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           }
         }
         const float ref = finite_or_zero(m);
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(-ref, -ref);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int c = 0; c < kTile; c += 32) {
           uint32_t packed[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float e0 = ex2(fmaf(x[c + 2 * i], p.scale_log2, -ref));
-            const float e1 = ex2(fmaf(x[c + 2 * i + 1], p.scale_log2, -ref));
-            sum[(2 * i) & 3] += e0;
-            sum[(2 * i + 1) & 3] += e1;
-            packed[i] = pack2<T>(e0, e1);   // weights rounded for the second product, their sum is not
+            float2 e = fma2(make_float2(x[c + 2 * i], x[c + 2 * i + 1]), scale2, shift2);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            sum[i & 1] = add2(sum[i & 1], e);
+            packed[i] = pack2<T>(e.x, e.y);   // weights rounded for the second product, their sum is not
           }
           tmem_st16(s_addr + c / 2, packed);
         }
-        l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        sum[0] = add2(sum[0], sum[1]);
+        l = l * alpha + (sum[0].x + sum[0].y);
         tc_wait_st();
         tc_fence_before();
         mbar_arrive(&sm.p_full[w]);
