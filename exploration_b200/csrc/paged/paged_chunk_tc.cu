@@ -18,11 +18,12 @@
 // through TMEM at the item's end. Either way the issuer alternates between the
 // warpgroups: while one exponentiates its scores, the other's products run.
 //
-// P (16 bit) overwrites its scores' TMEM columns. A running maximum is kept
-// until it grows by more than 2^8 (then O is rescaled in TMEM): S of step k + 2
-// is issued after P V of step k, so a finished S means a finished O.
+// P (16 bit) overwrites its scores' TMEM columns; steps use the score buffers in
+// turn (three at head dim 64, two at 128), so with three a warpgroup finds its
+// next scores ready. A running maximum is kept until it grows by more than 2^8
+// (then O is rescaled in TMEM).
 //
-// TMEM columns: S/P of warpgroup w at [128 w, 128 w + 128), O at [256 + D w, ...).
+// TMEM columns: score buffers from 0, then the two accumulators of D columns.
 //
 // Keys past an item's limit are masked, and their rows of the last V tile are
 // cleared in shared memory: a page's unwritten rows may hold anything.
@@ -53,12 +54,13 @@ constexpr float kRescale = 8.f;       // log2 units
 template <int D>
 struct alignas(1024) ChunkSmem {
   static constexpr int kStages = D == 64 ? 4 : 2;   // of each ring
+  static constexpr int kBufs = (kTmemCols - 2 * D) / 128;   // score buffers in TMEM
   uint16_t q[2][kM * D];
   uint16_t k[kStages][kTile * D];
   uint16_t v[kStages][kTile * D];
   uint64_t q_full, q_empty;
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[2], p_full[2], o_full[2], join;
+  uint64_t s_full[kBufs], p_full[kBufs], o_done[2], join;
   uint32_t tmem_base;
   int abort;
   float ml[kM][2];
@@ -83,6 +85,42 @@ EB_DEVICE void hold(uint32_t (&r)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 
+// True in one lane of a converged warp; unlike a comparison of lane numbers it
+// lets the compiler keep the operands of the guarded instructions uniform.
+EB_DEVICE bool elect_one() {
+  uint32_t pred;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
+  return pred != 0;
+}
+
+// Shared-memory matrix descriptors (128-byte swizzle, 1,024 bytes between groups of
+// eight rows) in two words: only the low one, address and leading offset, changes.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+
+EB_DEVICE uint32_t desc_lo(const void* ptr, uint32_t leading_bytes) {
+  return (smem_u32(ptr) >> 4) | ((leading_bytes >> 4) << 16);
+}
+
+template <uint32_t HI>
+EB_DEVICE void mma_ss_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(HI)
+      : "memory");
+}
+
+template <uint32_t HI>
+EB_DEVICE void mma_ts_lo(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(HI)
+      : "memory");
+}
+
+EB_DEVICE int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -90,7 +128,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   extern __shared__ __align__(1024) uint8_t raw_smem[];
   ChunkSmem<D>& sm = *reinterpret_cast<ChunkSmem<D>*>(
       (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  constexpr int kStages = ChunkSmem<D>::kStages;
+  constexpr int kStages = ChunkSmem<D>::kStages, kBufs = ChunkSmem<D>::kBufs;
+  constexpr int kO = kTmemCols - 2 * D;          // first TMEM column of the accumulators
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort = &sm.abort;
   if (threadIdx.x == 0) {
@@ -102,11 +141,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       mbar_init(&sm.v_full[s], 1);
       mbar_init(&sm.v_empty[s], 1);
     }
-    for (int w = 0; w < 2; ++w) {
-      mbar_init(&sm.s_full[w], 1);
-      mbar_init(&sm.p_full[w], 128);
-      mbar_init(&sm.o_full[w], 1);
+    for (int b = 0; b < kBufs; ++b) {
+      mbar_init(&sm.s_full[b], 1);
+      mbar_init(&sm.p_full[b], 128);
     }
+    mbar_init(&sm.o_done[0], 1);
+    mbar_init(&sm.o_done[1], 1);
     mbar_init(&sm.join, 256);
     sm.abort = 0;
     fence_barrier_init();
@@ -143,7 +183,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       finish_segment(p, s, lane);
       if (s.begin == s.end) continue;
       const int kv_head = s.head / p.head_div;
-      if (q_loads > 0 && !__all_sync(0xffffffffu, mbar_wait(&sm.q_empty, (q_loads - 1) & 1, abort, err, kSiteQFull)))
+      if (q_loads > 0 && !__all_sync(0xffffffffu, wait_tight(&sm.q_empty, (q_loads - 1) & 1, abort, err, kSiteQFull)))
         break;
       const int halves = split_rows(s) ? 2 : 1;
       if (lane == 0) {
@@ -182,7 +222,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           uint16_t* dst = part == 0 ? sm.k[ring.stage] : sm.v[ring.stage];
           const CUtensorMap* map = part == 0 ? &tk : &tv;
           if (tiles_issued >= kStages &&
-              !__all_sync(0xffffffffu, mbar_wait(empty, ring.phase ^ 1, abort, err, kSiteKvEmpty))) {
+              !__all_sync(0xffffffffu, wait_tight(empty, ring.phase ^ 1, abort, err, kSiteKvEmpty))) {
             ok = false;
             break;
           }
@@ -211,45 +251,45 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
     const uint32_t id_s = idesc_16(kBf16, kM, kTile, false, false);
     const uint32_t id_pv = idesc_16(kBf16, kM, D, false, true);
-    Ring kr, vr;
+    Ring kr, vr, sr, pr;    // key and value stages, score buffers to fill and weights to use
     int segments = 0;
-    uint32_t p_phase = 0;   // bit w: parity of warpgroup w's next weights
     bool ok = true;
     while (ok && walk.next(p, sm.cum, s)) {
       finish_segment(p, s, lane);
       if (s.begin == s.end) continue;
       const bool dual = split_rows(s);
       const int tiles = s.end - s.begin, steps = dual ? 2 * tiles : tiles;
-      if (!__all_sync(0xffffffffu, mbar_wait(&sm.q_full, segments & 1, abort, err, kSiteQFull))) break;
+      if (!__all_sync(0xffffffffu, wait_tight(&sm.q_full, segments & 1, abort, err, kSiteQFull))) break;
       ++segments;
       // Step i belongs to warpgroup i & 1; with rows of their own both take each tile.
       auto issue_s = [&](int i) -> bool {
         const int w = i & 1;
         if (!dual || w == 0) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&sm.k_full[kr.stage], kr.phase, abort, err, kSiteKvFull))) return false;
+          if (!__all_sync(0xffffffffu, wait_tight(&sm.k_full[kr.stage], kr.phase, abort, err, kSiteKvFull))) return false;
         }
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t q_addr = smem_u32(sm.q[dual ? w : 0]), k_addr = smem_u32(sm.k[kr.stage]);
+        const uint32_t q_lo = uniform(desc_lo(sm.q[dual ? w : 0], 16)), k_lo = uniform(desc_lo(sm.k[kr.stage], 16));
+        const uint32_t d_addr = uniform(tmem + sr.stage * 128);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = (kk / 4) * kBox * 2 + (kk % 4) * 32;
-            mma_ss(tmem + w * 128, smem_desc_sw128(q_addr + off, 16, 1024), smem_desc_sw128(k_addr + off, 16, 1024),
-                   id_s, kk > 0);
+            mma_ss_lo<kDescHi>(d_addr, q_lo + (off >> 4), k_lo + (off >> 4), id_s, kk > 0);
           }
-          tc_commit(&sm.s_full[w]);
+          tc_commit(&sm.s_full[sr.stage]);
           if (!dual || w == 1) tc_commit(&sm.k_empty[kr.stage]);
           if (i == steps - 1) tc_commit(&sm.q_empty);
         }
         __syncwarp();
+        sr.next(kBufs);
         if (!dual || w == 1) kr.next(kStages);
         return true;
       };
-      ok = issue_s(0) && (steps == 1 || issue_s(1));
+      for (int i = 0; ok && i < min(kBufs, steps); ++i) ok = issue_s(i);
       for (int i = 0; ok && i < steps; ++i) {
         const int w = i & 1, tile = s.begin + (dual ? i >> 1 : i);
         if (!dual || w == 0) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&sm.v_full[vr.stage], vr.phase, abort, err, kSiteKvFull))) {
+          if (!__all_sync(0xffffffffu, wait_tight(&sm.v_full[vr.stage], vr.phase, abort, err, kSiteKvFull))) {
             ok = false;
             break;
           }
@@ -263,24 +303,25 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             __syncwarp();
           }
         }
-        if (!__all_sync(0xffffffffu, mbar_wait(&sm.p_full[w], p_phase >> w & 1, abort, err, kSitePFull))) {
+        if (!__all_sync(0xffffffffu, wait_tight(&sm.p_full[pr.stage], pr.phase, abort, err, kSitePFull))) {
           ok = false;
           break;
         }
-        p_phase ^= 1u << w;
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t v_addr = smem_u32(sm.v[vr.stage]);
+        const uint32_t v_lo = uniform(desc_lo(sm.v[vr.stage], kBox * 2));
+        const uint32_t o_addr = uniform(tmem + kO + w * D), p_addr = uniform(tmem + pr.stage * 128);
+        const uint32_t more = uniform(i > 1);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kTile / 16; ++kk)
-            mma_ts(tmem + 256 + w * D, tmem + w * 128 + kk * 8, smem_desc_sw128(v_addr + kk * 2048, kBox * 2, 1024),
-                   id_pv, i > 1 || kk > 0);
+            mma_ts_lo<kDescHi>(o_addr, p_addr + kk * 8, v_lo + kk * (2048 >> 4), id_pv, kk > 0 ? 1u : more);
           if (!dual || w == 1) tc_commit(&sm.v_empty[vr.stage]);
-          if (i >= steps - 2) tc_commit(&sm.o_full[w]);
+          tc_commit(&sm.o_done[w]);
         }
         __syncwarp();
+        pr.next(kBufs);
         if (!dual || w == 1) vr.next(kStages);
-        if (i + 2 < steps) ok = issue_s(i + 2);
+        if (i + kBufs < steps) ok = issue_s(i + kBufs);
       }
     }
   }
@@ -289,14 +330,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     const int w = (warp >> 2) - 1;                   // softmax warpgroup
     const int row = (warp & 3) * 32 + lane;          // TMEM lane
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t s_addr = lane_addr + w * 128;
-    int steps_done = 0, segments = 0, joins = 0;
+    const uint32_t o_addr = lane_addr + kO + w * D;
+    int joins = 0;
+    uint32_t done = 0;       // products this warpgroup has asked for
+    uint32_t step0 = 0;      // steps of earlier items, both warpgroups'
     bool ok = true;
     // Both warpgroups, bounded: TMEM accesses before it are ordered before those after it.
     auto join = [&]() -> bool {
       tc_fence_before();
       mbar_arrive(&sm.join);
-      const bool met = __all_sync(0xffffffffu, mbar_wait(&sm.join, joins & 1, abort, err, kSiteODone));
+      const bool met = __all_sync(0xffffffffu, wait_tight(&sm.join, joins & 1, abort, err, kSiteODone));
       ++joins;
       tc_fence_after();
       return met;
@@ -315,11 +358,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       const int stride = dual ? 1 : 2;
       int begun = 0;
       for (int tile = s.begin + (dual ? 0 : w); tile < s.end; tile += stride, ++begun) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[w], steps_done & 1, abort, err, kSiteSFull))) {
+        const uint32_t step = step0 + (dual ? 2 * begun + w : tile - s.begin);
+        const uint32_t buf = step % kBufs;
+        const uint32_t s_addr = lane_addr + buf * 128;
+        if (!__all_sync(0xffffffffu, wait_tight(&sm.s_full[buf], step / kBufs & 1, abort, err, kSiteSFull))) {
           ok = false;
           break;
         }
-        ++steps_done;
         tc_fence_after();
         float x[kTile];
 #pragma unroll
@@ -353,15 +398,20 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           m = peak;
         }
         if (begun > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+          if (!__all_sync(0xffffffffu, wait_tight(&sm.o_done[w], (done - 1) & 1, abort, err, kSiteODone))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
 #pragma unroll
           for (int c = 0; c < D; c += 16) {
             uint32_t r[16];
-            tmem_ld16(lane_addr + 256 + w * D + c, r);
+            tmem_ld16(o_addr + c, r);
             tc_wait_ld();
             hold(r);
 #pragma unroll
             for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-            tmem_st16(lane_addr + 256 + w * D + c, r);
+            tmem_st16(o_addr + c, r);
           }
         }
         const float ref = finite_or_zero(m);
@@ -384,12 +434,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         l = l * alpha + (sum[0].x + sum[0].y);
         tc_wait_st();
         tc_fence_before();
-        mbar_arrive(&sm.p_full[w]);
+        mbar_arrive(&sm.p_full[buf]);
+        ++done;
       }
       if (!ok) break;
+      step0 += (dual ? 2 : 1) * (s.end - s.begin);
       if (begun > 0) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&sm.o_full[w], segments & 1, abort, err, kSiteODone))) break;
-        ++segments;
+        if (!__all_sync(0xffffffffu, wait_tight(&sm.o_done[w], (done - 1) & 1, abort, err, kSiteODone))) break;
         tc_fence_after();
       }
       if (pos < 0) {   // a padding row: zero, no weight
@@ -429,7 +480,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           float o[32];
           uint32_t r[32];
           if (s.begin < s.end) {
-            tmem_ld32(lane_addr + 256 + w * D + c, r);
+            tmem_ld32(o_addr + c, r);
             tc_wait_ld();
             hold(r);
 #pragma unroll
@@ -439,7 +490,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             for (int i = 0; i < 32; ++i) o[i] = 0.f;
           }
           if (two) {
-            tmem_ld32(lane_addr + 256 + D + c, r);
+            tmem_ld32(o_addr + D + c, r);
             tc_wait_ld();
             hold(r);
 #pragma unroll

@@ -4,7 +4,7 @@
 
 #include <type_traits>
 
-#include "../common/util.cuh"
+#include "../common/sm100.cuh"
 
 namespace eb {
 namespace paged {
@@ -47,6 +47,25 @@ EB_DEVICE uint32_t pack2(float lo, float hi) {
   } else {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// Bounded wait of the tile loops: sm100::mbar_wait without its sleep between
+// polls (the poll itself suspends the warp for a while); the time and the abort
+// word are looked at every 32 polls.
+EB_DEVICE bool wait_tight(uint64_t* bar, uint32_t parity, volatile int* abort, sm100::ErrorSlot* err, int site) {
+  if (sm100::mbar_try_wait(bar, parity)) return true;
+  const long long start = clock64();
+  for (int i = 1;; ++i) {
+    if (sm100::mbar_try_wait(bar, parity)) return true;
+    if ((i & 31) == 0) {
+      if (*abort) return false;
+      if (clock64() - start > 2000000000LL) {   // about a second
+        *abort = 1;
+        sm100::report(err, site);
+        return false;
+      }
+    }
   }
 }
 

@@ -105,7 +105,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       int ids = entry(base + lane), ahead = entry(base + 32 + lane);
       for (int tile = s.begin; tile < s.end; ++tile) {
         const int stage = issued % kStages;
-        if (issued >= kStages && !__all_sync(0xffffffffu, mbar_wait(&sm.empty[stage], ((issued / kStages) - 1) & 1,
+        if (issued >= kStages && !__all_sync(0xffffffffu, wait_tight(&sm.empty[stage], ((issued / kStages) - 1) & 1,
                                                                     abort, err, kSiteKvEmpty))) {
           ok = false;
           break;
@@ -186,7 +186,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
     for (int tile = s.begin; tile < s.end; ++tile, ++done) {
       const int stage = done % kStages;
-      if (!__all_sync(0xffffffffu, mbar_wait(&sm.full[stage], (done / kStages) & 1, abort, err, kSiteKvFull))) {
+      if (!__all_sync(0xffffffffu, wait_tight(&sm.full[stage], (done / kStages) & 1, abort, err, kSiteKvFull))) {
         ok = false;
         break;
       }
