@@ -11,6 +11,7 @@
 //                128-byte swizzle) into two rings
 //   warp 1       MMA issuer: S = Q K^T into TMEM, O += P V with P read from TMEM
 //   warp 2       TMEM owner (512 columns)
+//   warp 3       clears the rows past an item's limit in its last V tile
 //   warps 4-7    softmax warpgroup 0, one thread a row (TMEM lane)
 //   warps 8-11   softmax warpgroup 1
 // Items of more than 128 rows give each warpgroup its own 128 rows of every key
@@ -25,8 +26,8 @@
 //
 // TMEM columns: score buffers from 0, then the two accumulators of D columns.
 //
-// Keys past an item's limit are masked, and their rows of the last V tile are
-// cleared in shared memory: a page's unwritten rows may hold anything.
+// Keys past an item's limit are masked, and their V rows cleared: a page's
+// unwritten rows may hold anything.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 
@@ -60,9 +61,10 @@ struct alignas(1024) ChunkSmem {
   uint16_t v[kStages][kTile * D];
   uint64_t q_full, q_empty;
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[kBufs], p_full[kBufs], o_done[2], join;
+  uint64_t s_full[kBufs], p_full[kBufs], o_done[2], join, v_ragged, v_clear;
   uint32_t tmem_base;
   int abort;
+  int clear_stage;
   float ml[kM][2];
   int cum[kMaxEntries + 1];
 };
@@ -119,8 +121,6 @@ EB_DEVICE void mma_ts_lo(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32
       : "memory");
 }
 
-EB_DEVICE int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -148,6 +148,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     mbar_init(&sm.o_done[0], 1);
     mbar_init(&sm.o_done[1], 1);
     mbar_init(&sm.join, 256);
+    mbar_init(&sm.v_ragged, 1);
+    mbar_init(&sm.v_clear, 1);
     sm.abort = 0;
     fence_barrier_init();
   }
@@ -252,77 +254,89 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     const uint32_t id_s = idesc_16(kBf16, kM, kTile, false, false);
     const uint32_t id_pv = idesc_16(kBf16, kM, D, false, true);
     Ring kr, vr, sr, pr;    // key and value stages, score buffers to fill and weights to use
-    int segments = 0;
+    int segments = 0, cleared = 0;
     bool ok = true;
     while (ok && walk.next(p, sm.cum, s)) {
       finish_segment(p, s, lane);
       if (s.begin == s.end) continue;
       const bool dual = split_rows(s);
       const int tiles = s.end - s.begin, steps = dual ? 2 * tiles : tiles;
-      if (!__all_sync(0xffffffffu, wait_tight(&sm.q_full, segments & 1, abort, err, kSiteQFull))) break;
+      const int ragged = s.limit < s.end * kTile ? s.end - 1 : -1;   // tile whose values warp 3 clears
+      const int q_phase = segments & 1, clear_phase = cleared & 1;
       ++segments;
-      // Step i belongs to warpgroup i & 1; with rows of their own both take each tile.
-      auto issue_s = [&](int i) -> bool {
-        const int w = i & 1;
-        if (!dual || w == 0) {
-          if (!__all_sync(0xffffffffu, wait_tight(&sm.k_full[kr.stage], kr.phase, abort, err, kSiteKvFull))) return false;
-        }
-        tc_fence_after();
-        const uint32_t q_lo = uniform(desc_lo(sm.q[dual ? w : 0], 16)), k_lo = uniform(desc_lo(sm.k[kr.stage], 16));
-        const uint32_t d_addr = uniform(tmem + sr.stage * 128);
-        if (elect_one()) {
+      cleared += ragged >= 0;
+      // One thread does all of an item: a warp-wide wait costs a vote, and there are three a step.
+      if (elect_one()) {
+        // Step i belongs to warpgroup i & 1; with rows of their own both take each tile.
+        auto issue_s = [&](int i) {
+          const int w = i & 1;
+          if (!dual || w == 0) ok = ok && wait_tight(&sm.k_full[kr.stage], kr.phase, abort, err, kSiteKvFull);
+          if (!ok) return;
+          tc_fence_after();
+          const uint32_t q_lo = desc_lo(sm.q[dual ? w : 0], 16), k_lo = desc_lo(sm.k[kr.stage], 16);
+          const uint32_t d_addr = tmem + sr.stage * 128;
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = (kk / 4) * kBox * 2 + (kk % 4) * 32;
             mma_ss_lo<kDescHi>(d_addr, q_lo + (off >> 4), k_lo + (off >> 4), id_s, kk > 0);
           }
           tc_commit(&sm.s_full[sr.stage]);
-          if (!dual || w == 1) tc_commit(&sm.k_empty[kr.stage]);
           if (i == steps - 1) tc_commit(&sm.q_empty);
-        }
-        __syncwarp();
-        sr.next(kBufs);
-        if (!dual || w == 1) kr.next(kStages);
-        return true;
-      };
-      for (int i = 0; ok && i < min(kBufs, steps); ++i) ok = issue_s(i);
-      for (int i = 0; ok && i < steps; ++i) {
-        const int w = i & 1, tile = s.begin + (dual ? i >> 1 : i);
-        if (!dual || w == 0) {
-          if (!__all_sync(0xffffffffu, wait_tight(&sm.v_full[vr.stage], vr.phase, abort, err, kSiteKvFull))) {
-            ok = false;
-            break;
+          sr.next(kBufs);
+          if (!dual || w == 1) {
+            tc_commit(&sm.k_empty[kr.stage]);
+            kr.next(kStages);
           }
-          const int valid = s.limit - tile * kTile;
-          if (valid < kTile) {   // rows past the limit: cleared once, before the first product that reads them
-            uint4* rows = reinterpret_cast<uint4*>(sm.v[vr.stage]);
-            for (int j = valid * 8 + lane; j < kTile * 8; j += 32)
-#pragma unroll
-              for (int h = 0; h < D / 64; ++h) rows[h * (kBox / 8) + j] = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
-            __syncwarp();
+        };
+        ok = wait_tight(&sm.q_full, q_phase, abort, err, kSiteQFull);
+        for (int i = 0; ok && i < min(kBufs, steps); ++i) issue_s(i);
+        for (int i = 0; ok && i < steps; ++i) {
+          const int w = i & 1, tile = s.begin + (dual ? i >> 1 : i);
+          if (!dual || w == 0) {
+            ok = wait_tight(&sm.v_full[vr.stage], vr.phase, abort, err, kSiteKvFull);
+            if (ok && tile == ragged) {
+              sm.clear_stage = vr.stage;
+              mbar_arrive(&sm.v_ragged);
+              ok = wait_tight(&sm.v_clear, clear_phase, abort, err, kSiteKvFull);
+            }
           }
-        }
-        if (!__all_sync(0xffffffffu, wait_tight(&sm.p_full[pr.stage], pr.phase, abort, err, kSitePFull))) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t v_lo = uniform(desc_lo(sm.v[vr.stage], kBox * 2));
-        const uint32_t o_addr = uniform(tmem + kO + w * D), p_addr = uniform(tmem + pr.stage * 128);
-        const uint32_t more = uniform(i > 1);
-        if (elect_one()) {
+          ok = ok && wait_tight(&sm.p_full[pr.stage], pr.phase, abort, err, kSitePFull);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t v_lo = desc_lo(sm.v[vr.stage], kBox * 2);
+          const uint32_t o_addr = tmem + kO + w * D, p_addr = tmem + pr.stage * 128, more = i > 1;
 #pragma unroll
           for (int kk = 0; kk < kTile / 16; ++kk)
             mma_ts_lo<kDescHi>(o_addr, p_addr + kk * 8, v_lo + kk * (2048 >> 4), id_pv, kk > 0 ? 1u : more);
-          if (!dual || w == 1) tc_commit(&sm.v_empty[vr.stage]);
           tc_commit(&sm.o_done[w]);
+          pr.next(kBufs);
+          if (!dual || w == 1) {
+            tc_commit(&sm.v_empty[vr.stage]);
+            vr.next(kStages);
+          }
+          if (i + kBufs < steps) issue_s(i + kBufs);
         }
-        __syncwarp();
-        pr.next(kBufs);
-        if (!dual || w == 1) vr.next(kStages);
-        if (i + kBufs < steps) ok = issue_s(i + kBufs);
       }
+      ok = __all_sync(0xffffffffu, ok);
+    }
+  } else if (warp == 3) {
+    // Rows past an item's limit in its last value tile: cleared when warp 1 has seen the tile arrive.
+    int cleared = 0;
+    bool ok = true;
+    while (ok && walk.next(p, sm.cum, s)) {
+      finish_segment(p, s, lane);
+      if (s.begin == s.end || s.limit >= s.end * kTile) continue;
+      ok = __all_sync(0xffffffffu, mbar_wait(&sm.v_ragged, cleared & 1, abort, err, kSiteKvFull));
+      if (!ok) break;
+      ++cleared;
+      const int stage = *static_cast<volatile int*>(&sm.clear_stage);
+      uint4* rows = reinterpret_cast<uint4*>(sm.v[stage]);
+      for (int j = (s.limit - (s.end - 1) * kTile) * 8 + lane; j < kTile * 8; j += 32)
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) rows[h * (kBox / 8) + j] = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.v_clear);
     }
   }
   } else {

@@ -189,13 +189,20 @@ EB_DEVICE void publish_run(const Args& p, const int* cum, const Walk& walk) {
     reinterpret_cast<int4*>(p.cuts)[blockIdx.x] = cut;
     if (blockIdx.x == 0) *p.run = static_cast<int>(run_tiles(p, cum[p.batch * p.row_tiles], gridDim.x));
   }
+  // Every CTA takes a share of each such entry: the last tiles of a ragged batch may all be empty.
   const int entries = p.batch * p.row_tiles;
-  for (int e = blockIdx.x; e < entries; e += gridDim.x) {
+  const int64_t row = static_cast<int64_t>(p.heads) * p.dim * sizeof(T);
+  const int64_t at = blockIdx.x * blockDim.x + threadIdx.x, step = gridDim.x * blockDim.x;
+  for (int e = 0; e < entries; ++e) {
     if (cum[e + 1] != cum[e]) continue;
     const int b = e / p.row_tiles, t0 = (e - b * p.row_tiles) * p.tile_tokens;
-    const int64_t n = static_cast<int64_t>(min(p.tile_tokens, p.tokens - t0)) * p.heads * p.dim;
-    T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.tokens + t0) * p.heads * p.dim;
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) out[i] = cast_f<T>(0.f);
+    const int64_t n = min(p.tile_tokens, p.tokens - t0) * row;
+    char* out = static_cast<char*>(p.out) + (static_cast<int64_t>(b) * p.tokens + t0) * row;
+    if (row % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0) {
+      for (int64_t i = at * 16; i < n; i += step * 16) *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
+    } else {   // an even number of elements of two bytes or more
+      for (int64_t i = at * 4; i < n; i += step * 4) *reinterpret_cast<uint32_t*>(out + i) = 0;
+    }
   }
 }
 
