@@ -17,6 +17,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include "../common/checks.h"
 #include "../common/util.cuh"
 
 namespace eb {
@@ -83,9 +84,27 @@ beam_reorder_kernel(ReorderArgs p) {
 
 }  // namespace
 
-std::vector<at::Tensor> beam_reorder(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& tables,
-                                     const at::Tensor& spare, const at::Tensor& parents, const at::Tensor& lengths) {
+std::tuple<at::Tensor, at::Tensor> beam_reorder(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& tables_in,
+                                                const at::Tensor& spare_in, const at::Tensor& parents_in,
+                                                const at::Tensor& lengths_in) {
+  // The Python module makes the same checks for CPU tensors, with the same messages.
+  TORCH_CHECK_VALUE(k_cache.dim() == 5 && k_cache.sizes() == v_cache.sizes() && tables_in.dim() == 3 &&
+                        spare_in.dim() == 2 && spare_in.size(0) == tables_in.size(0) &&
+                        spare_in.size(1) == tables_in.size(1) && parents_in.sizes() == spare_in.sizes() &&
+                        lengths_in.dim() == 1 && lengths_in.size(0) == spare_in.size(0) && tables_in.size(2) >= 1,
+                    "expected pools [layers, pages, kv_heads, page, head_dim], tables [groups, beams, width], "
+                    "spare, parents [groups, beams] and lengths [groups]");
+  TORCH_CHECK_VALUE(k_cache.scalar_type() == v_cache.scalar_type() && k_cache.element_size() % 2 == 0,
+                    "key and value pools must have one dtype of 16 bits or more");
+  TORCH_CHECK_VALUE(tables_in.scalar_type() == at::kInt && spare_in.scalar_type() == at::kInt &&
+                        lengths_in.scalar_type() == at::kInt && parents_in.scalar_type() == at::kLong,
+                    "tables, spare and lengths must be int32 and parents int64");
+  TORCH_CHECK_VALUE(same_device(k_cache, v_cache, tables_in, spare_in, parents_in, lengths_in),
+                    "all tensors must be on one device");
+  TORCH_CHECK_VALUE(k_cache.is_contiguous() && v_cache.is_contiguous(), "cache pools must be contiguous");
   c10::cuda::CUDAGuard guard(k_cache.device());
+  const at::Tensor tables = tables_in.contiguous(), spare = spare_in.contiguous(), parents = parents_in.contiguous(),
+                   lengths = lengths_in.contiguous();
   at::Tensor tables_out = at::empty_like(tables), spare_out = at::empty_like(spare);
   const int64_t slots = spare.numel(), layers = k_cache.size(0);
   if (slots == 0) return {tables_out, spare_out};

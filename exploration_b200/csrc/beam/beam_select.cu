@@ -21,6 +21,7 @@
 
 #include <climits>
 
+#include "../common/checks.h"
 #include "../common/util.cuh"
 
 namespace eb {
@@ -323,12 +324,10 @@ void launch(SelectArgs& args, int groups, const at::TensorOptions& f32, cudaStre
   const int64_t rows = static_cast<int64_t>(groups) * args.beams;
   // One chunk more than the vocabulary needs when the row starts inside a vector.
   args.chunks = cdiv(args.vocab + 16 / static_cast<int>(sizeof(T)) - 1, kChunk);
-  at::Tensor ms = at::empty({rows, args.chunks, 2}, f32);
-  at::Tensor x = at::empty({rows, args.chunks, args.keep}, f32);
-  at::Tensor t = at::empty({rows, args.chunks, args.keep}, f32.dtype(at::kInt));
-  args.part_ms = ms.data_ptr<float>();
-  args.part_x = x.data_ptr<float>();
-  args.part_t = t.data_ptr<int>();
+  at::Tensor space = at::empty({rows * args.chunks * (2 + 2 * args.keep)}, f32);
+  args.part_ms = space.data_ptr<float>();
+  args.part_x = args.part_ms + rows * args.chunks * 2;
+  args.part_t = reinterpret_cast<int*>(args.part_x + rows * args.chunks * args.keep);
   beam_select_chunk_kernel<T><<<dim3(args.chunks, rows), kChunkWarps * 32, 0, stream>>>(args);
   EB_CUDA_CHECK(cudaGetLastError());
   cudaLaunchConfig_t config = {};
@@ -346,15 +345,29 @@ void launch(SelectArgs& args, int groups, const at::TensorOptions& f32, cudaStre
 
 }  // namespace
 
-std::vector<at::Tensor> beam_select(const at::Tensor& logits, const at::Tensor& scores, const at::Tensor& finished,
-                                    int64_t eos) {
-  c10::cuda::CUDAGuard guard(logits.device());
-  const int64_t groups = logits.size(0), beams = logits.size(1), vocab = logits.size(2);
-  TORCH_CHECK(beams <= kMaxBeams, "beam_select: at most ", kMaxBeams, " beams");
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> beam_select(const at::Tensor& logits_in,
+                                                                       const at::Tensor& scores_in,
+                                                                       const at::Tensor& finished_in, int64_t eos) {
+  // The Python module makes the same checks for CPU tensors, with the same messages.
+  TORCH_CHECK_VALUE(logits_in.dim() == 3 && scores_in.dim() == 2 && scores_in.size(0) == logits_in.size(0) &&
+                        scores_in.size(1) == logits_in.size(1) && finished_in.sizes() == scores_in.sizes(),
+                    "expected logits [groups, beams, vocab] and scores, finished [groups, beams]");
+  TORCH_CHECK_VALUE(scores_in.scalar_type() == at::kFloat && finished_in.scalar_type() == at::kBool,
+                    "scores must be fp32 and finished bool");
+  TORCH_CHECK_VALUE(same_device(logits_in, scores_in, finished_in), "all tensors must be on one device");
+  const int64_t groups = logits_in.size(0), beams = logits_in.size(1), vocab = logits_in.size(2);
+  static_assert(kMaxBeams == 32);
+  TORCH_CHECK_VALUE(beams >= 1 && beams <= kMaxBeams && vocab >= 1, "between 1 and 32 beams and at least one token");
+  TORCH_CHECK_VALUE(!wants_grad(logits_in) && !wants_grad(scores_in),
+                    "beam_select is for inference: it has no gradient");
+  TORCH_CHECK_VALUE(eos >= -1 && eos < vocab, "eos must be a token or -1");
+  TORCH_CHECK_VALUE(native_dtype(logits_in), "the native selection takes fp32, fp16 or bf16 logits");
   TORCH_CHECK(groups * beams < 65536 && vocab < (1LL << 30), "beam_select: too many rows or tokens");
+  c10::cuda::CUDAGuard guard(logits_in.device());
+  const at::Tensor logits = logits_in.contiguous(), scores = scores_in.contiguous(), finished = finished_in.contiguous();
   at::Tensor scores_out = at::empty_like(scores);
-  at::Tensor parents = at::empty({groups, beams}, scores.options().dtype(at::kLong));
-  at::Tensor tokens = at::empty_like(parents);
+  at::Tensor both = at::empty({2, groups, beams}, scores.options().dtype(at::kLong));
+  at::Tensor parents = both.select(0, 0), tokens = both.select(0, 1);
   at::Tensor finished_out = at::empty_like(finished);
   if (groups * beams > 0) {
     SelectArgs args{};

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <string>
+#include <tuple>
 #include <vector>
 
 namespace eb {
@@ -106,10 +107,12 @@ at::Tensor paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tens
 std::string paged_attention_path(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache);
 at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
                            const at::Tensor& tables, const at::Tensor& positions);
-std::vector<at::Tensor> beam_select(const at::Tensor& logits, const at::Tensor& scores, const at::Tensor& finished,
-                                    int64_t eos);
-std::vector<at::Tensor> beam_reorder(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& tables,
-                                     const at::Tensor& spare, const at::Tensor& parents, const at::Tensor& lengths);
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> beam_select(const at::Tensor& logits,
+                                                                       const at::Tensor& scores,
+                                                                       const at::Tensor& finished, int64_t eos);
+std::tuple<at::Tensor, at::Tensor> beam_reorder(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& tables,
+                                                const at::Tensor& spare, const at::Tensor& parents,
+                                                const at::Tensor& lengths);
 }  // namespace eb
 
 namespace {

@@ -16,6 +16,7 @@
 #include <torch/extension.h>
 
 #include "../common/util.cuh"
+#include "paged_checks.h"
 
 namespace eb {
 namespace {
@@ -111,10 +112,24 @@ void launch(const AppendArgs& args, int64_t count, cudaStream_t stream) {
 
 }  // namespace
 
-at::Tensor paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cos,
-                        const at::Tensor& sin, at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& tables,
-                        const at::Tensor& positions) {
-  c10::cuda::CUDAGuard guard(q.device());
+at::Tensor paged_append(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+                        const at::Tensor& cos_in, const at::Tensor& sin_in, at::Tensor& k_cache, at::Tensor& v_cache,
+                        const at::Tensor& tables_in, const at::Tensor& positions_in) {
+  paged::check_cache(q_in, k_cache, v_cache, tables_in, positions_in);
+  TORCH_CHECK_VALUE(k_in.sizes() == v_in.sizes() && k_in.dim() == 4 && k_in.size(0) == q_in.size(0) &&
+                        k_in.size(1) == q_in.size(1) && k_in.size(2) == k_cache.size(1) && k_in.size(3) == q_in.size(3),
+                    "expected k, v [batch, tokens, kv_heads, head_dim]");
+  TORCH_CHECK_VALUE(k_in.scalar_type() == q_in.scalar_type() && v_in.scalar_type() == q_in.scalar_type() &&
+                        same_device(q_in, k_in, v_in, cos_in, sin_in),
+                    "queries, keys, values and rotation tables must match in dtype and device");
+  TORCH_CHECK_VALUE(cos_in.sizes() == sin_in.sizes() && cos_in.dim() == 2 && cos_in.size(1) * 2 == q_in.size(3) &&
+                        cos_in.scalar_type() == at::kFloat && sin_in.scalar_type() == at::kFloat,
+                    "expected fp32 cos, sin [positions, head_dim / 2]");
+  TORCH_CHECK_VALUE(!wants_grad(k_in) && !wants_grad(v_in), "paged operators are for inference: they have no gradient");
+  c10::cuda::CUDAGuard guard(q_in.device());
+  auto rows = [](const at::Tensor& t) { return t.stride(3) == 1 ? t : t.contiguous(); };
+  const at::Tensor q = rows(q_in), k = rows(k_in), v = rows(v_in), cos = cos_in.contiguous(), sin = sin_in.contiguous();
+  const at::Tensor tables = tables_in.contiguous(), positions = paged::int32(positions_in);
   const int64_t batch = q.size(0), tokens = q.size(1), heads = q.size(2), dim = q.size(3);
   at::Tensor out = at::empty({batch, tokens, heads, dim}, q.options());
   if (batch * tokens == 0) return out;

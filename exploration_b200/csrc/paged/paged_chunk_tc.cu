@@ -538,14 +538,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
 
 template <typename T, int D>
 void launch(Args& args, int sms, cudaStream_t stream) {
-  const Split split(args, sms, stream);
+  const Split split(args, sms, 0);
   constexpr bool kHalf = std::is_same_v<T, __half>;
   const CUtensorMap tq = make_query_map(args, kHalf, kM / args.group);
   const CUtensorMap tk = make_pool_map(args, args.k, kHalf, kTile);
   const CUtensorMap tv = make_pool_map(args, args.v, kHalf, kTile);
   const size_t smem = sizeof(ChunkSmem<D>) + 1024;
   auto kernel = paged_chunk_kernel<T, D>;
-  EB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  allow_smem(reinterpret_cast<const void*>(kernel), smem);
   kernel<<<split.ctas, kThreads, smem, stream>>>(tq, tk, tv, args, device_error_slot(at::cuda::current_device()));
   EB_CUDA_CHECK(cudaGetLastError());
   count_launch(1);

@@ -4,6 +4,7 @@
 
 #include <string>
 
+#include "paged_checks.h"
 #include "paged_launch.h"
 
 namespace eb {
@@ -42,9 +43,11 @@ std::string paged_attention_path(const at::Tensor& q, const at::Tensor& k_cache,
   return path == Path::kRows ? "rows" : path == Path::kChunk ? "tcgen05" : "cuda_core";
 }
 
-at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
-                           const at::Tensor& tables, const at::Tensor& positions) {
-  c10::cuda::CUDAGuard guard(q.device());
+at::Tensor paged_attention(const at::Tensor& q_in, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                           const at::Tensor& tables_in, const at::Tensor& positions_in) {
+  paged::check_cache(q_in, k_cache, v_cache, tables_in, positions_in);
+  c10::cuda::CUDAGuard guard(q_in.device());
+  const at::Tensor q = q_in.contiguous(), tables = tables_in.contiguous(), positions = paged::int32(positions_in);
   at::Tensor out = at::empty_like(q);
   if (q.numel() == 0) return out;
   TORCH_CHECK(q.size(0) * q.size(1) * q.size(2) < (1LL << 31), "paged_attention: too many rows");

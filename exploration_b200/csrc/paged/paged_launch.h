@@ -5,6 +5,9 @@
 #include <ATen/cuda/CUDAContext.h>
 
 #include <algorithm>
+#include <mutex>
+#include <set>
+#include <utility>
 
 #include "../common/tma.cuh"
 #include "paged_common.cuh"
@@ -55,6 +58,15 @@ inline CUtensorMap make_query_map(const Args& args, bool half, int tokens) {
   return map;
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory, once per kernel and device.
+inline void allow_smem(const void* kernel, size_t bytes) {
+  static std::mutex mutex;
+  static std::set<std::pair<const void*, int>> done;
+  std::lock_guard<std::mutex> lock(mutex);
+  if (done.insert({kernel, at::cuda::current_device()}).second)
+    EB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+}
+
 // Row tiles of at most `most` rows: whole tokens of a group; a group that is
 // larger is divided into equal parts, each an item of its own.
 inline void set_rows(Args& args, int most, int key_tile) {
@@ -76,27 +88,28 @@ inline void set_rows(Args& args, int most, int key_tile) {
 // when the call has been enqueued.
 struct Split {
   int ctas = 0;
-  at::Tensor part_o, part_ml, cuts;
+  at::Tensor space;
 
-  Split(Args& args, int wanted, cudaStream_t) {
+  // `whole_tiles`: items of at most so many key tiles are not cut.
+  Split(Args& args, int wanted, int whole_tiles) {
     const int64_t entries = static_cast<int64_t>(args.batch) * args.row_tiles;
     const int64_t items = entries * args.item_heads;
-    args.flat = entries <= kMaxEntries;
+    const int64_t longest = cdiv64(static_cast<int64_t>(args.width) * args.page, args.key_tile);
+    args.flat = entries <= kMaxEntries && longest > whole_tiles;
     if (!args.flat) {
       TORCH_CHECK(items < (1LL << 31), "paged_attention: too many rows");
       ctas = static_cast<int>(items);
       return;
     }
-    const int64_t longest = cdiv64(static_cast<int64_t>(args.width) * args.page, args.key_tile);
     ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(wanted, items * longest)));
-    auto f32 = at::TensorOptions().device(at::kCUDA, at::cuda::current_device()).dtype(at::kFloat);
-    part_o = at::empty({2LL * ctas, args.row_tile, args.dim}, f32);
-    part_ml = at::empty({2LL * ctas, args.row_tile, 2}, f32);
-    cuts = at::empty({4LL * ctas + 1}, f32.dtype(at::kInt));
-    args.part_o = part_o.data_ptr<float>();
-    args.part_ml = part_ml.data_ptr<float>();
-    args.cuts = cuts.data_ptr<int>();
-    args.run = args.cuts + 4LL * ctas;
+    // One allocation: partial vectors, statistics, cuts.
+    const int64_t rows = 2LL * ctas * args.row_tile;
+    space = at::empty({rows * (args.dim + 2) + 4LL * ctas + 1},
+                      at::TensorOptions().device(at::kCUDA, at::cuda::current_device()).dtype(at::kFloat));
+    args.cuts = reinterpret_cast<int*>(space.data_ptr<float>());   // 16-byte entries first
+    args.part_o = space.data_ptr<float>() + 4LL * ctas;
+    args.part_ml = args.part_o + rows * args.dim;
+    args.run = reinterpret_cast<int*>(args.part_ml + rows * 2);
   }
 
   static int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }

@@ -33,6 +33,7 @@ using namespace sm100;
 
 constexpr int kRows = 16;
 constexpr int kTile = 64;
+constexpr int kWholeTiles = 16;   // items of up to 1,024 keys are not cut: joining costs a launch
 constexpr int kConsumers = 4;
 constexpr int kThreads = 32 * (kConsumers + 1);
 
@@ -329,12 +330,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 
 template <typename T, int D>
 void launch(Args& args, int sms, cudaStream_t stream) {
-  const Split split(args, sms * RowsConfig<D>::kCtas, stream);
+  const Split split(args, sms * RowsConfig<D>::kCtas, kWholeTiles);
   const CUtensorMap tk = make_pool_map(args, args.k, std::is_same_v<T, __half>, kTile);
   const CUtensorMap tv = make_pool_map(args, args.v, std::is_same_v<T, __half>, kTile);
   const size_t smem = sizeof(RowsSmem<D>) + 1024;
   auto kernel = paged_rows_kernel<T, D>;
-  EB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  allow_smem(reinterpret_cast<const void*>(kernel), smem);
   kernel<<<split.ctas, kThreads, smem, stream>>>(tk, tv, args, device_error_slot(at::cuda::current_device()));
   EB_CUDA_CHECK(cudaGetLastError());
   count_launch(1);

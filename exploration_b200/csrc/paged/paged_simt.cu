@@ -26,6 +26,7 @@ using namespace paged;
 
 constexpr int kWarps = 4;
 constexpr int kTile = 64;
+constexpr int kWholeTiles = 16;   // items of up to 1,024 keys are not cut: joining costs a launch
 constexpr int kWarpKeys = kTile / kWarps;
 
 template <typename T, int VE>
@@ -211,7 +212,7 @@ paged_simt_kernel(Args p) {
 
 template <typename T, int DP, int R>
 void launch(Args& args, int sms, cudaStream_t stream) {
-  const Split split(args, sms * 4, stream);
+  const Split split(args, sms * 4, kWholeTiles);
   paged_simt_kernel<T, DP, R><<<split.ctas, kWarps * 32, 0, stream>>>(args);
   EB_CUDA_CHECK(cudaGetLastError());
   count_launch(1);

@@ -8,8 +8,9 @@
   belongs to one beam, full pages are shared and never written again; every
   beam holds one spare page.
 
-Both are for inference. CUDA tensors run the sm_100a kernels of
-``csrc/beam``; CPU tensors run the definitions below.
+Both are for inference. CUDA tensors run the sm_100a kernels of ``csrc/beam``
+(the extension makes the checks that the functions here make for CPU tensors);
+CPU tensors run the definitions below.
 """
 from __future__ import annotations
 
@@ -17,10 +18,9 @@ import torch
 
 from . import _native
 from .gated_reference import NEG_INF, work_dtype
-from .launch import record
+from .launch import count
 
 MAX_BEAMS = 32
-LOGIT_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def beam_select(logits, scores, finished, eos):
@@ -35,6 +35,10 @@ def beam_select(logits, scores, finished, eos):
     ``tokens`` are int64; ``finished`` is true for an ended parent or token
     ``eos`` (``-1``: no token ends a beam).
     """
+    if logits.is_cuda:
+        out = _native.native(logits).beam_select(logits, scores, finished, eos)
+        count("beam_select", ("dtype", "beams"), (logits.dtype, logits.shape[1]))
+        return out
     if logits.ndim != 3 or scores.shape != logits.shape[:2] or finished.shape != scores.shape:
         raise ValueError("expected logits [groups, beams, vocab] and scores, finished [groups, beams]")
     if scores.dtype != torch.float32 or finished.dtype != torch.bool:
@@ -48,12 +52,6 @@ def beam_select(logits, scores, finished, eos):
     eos = int(eos)
     if not -1 <= eos < logits.shape[2]:
         raise ValueError("eos must be a token or -1")
-    if logits.is_cuda:
-        if logits.dtype not in LOGIT_DTYPES:
-            raise ValueError("the native selection takes fp32, fp16 or bf16 logits")
-        out = _native.native(logits).beam_select(logits.contiguous(), scores.contiguous(), finished.contiguous(), eos)
-        record("beam_select", dtype=str(logits.dtype), beams=logits.shape[1])
-        return tuple(out)
     return select_reference(logits, scores, finished, eos)
 
 
@@ -68,6 +66,10 @@ def beam_reorder(k_cache, v_cache, tables, spare, parents, lengths):
     beam; that page takes its place in the new table and the old one becomes
     the spare. The given tables are left as they are.
     """
+    if k_cache.is_cuda:
+        out = _native.native(k_cache).beam_reorder(k_cache, v_cache, tables, spare, parents, lengths)
+        count("beam_reorder", ("dtype", "page"), (k_cache.dtype, k_cache.shape[3]))
+        return out
     if k_cache.ndim != 5 or k_cache.shape != v_cache.shape or tables.ndim != 3 or spare.shape != tables.shape[:2] \
             or parents.shape != spare.shape or lengths.shape != spare.shape[:1] or tables.shape[2] < 1:
         raise ValueError("expected pools [layers, pages, kv_heads, page, head_dim], tables [groups, beams, width], "
@@ -81,11 +83,6 @@ def beam_reorder(k_cache, v_cache, tables, spare, parents, lengths):
         raise ValueError("all tensors must be on one device")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("cache pools must be contiguous")
-    if k_cache.is_cuda:
-        out = _native.native(k_cache).beam_reorder(k_cache, v_cache, tables.contiguous(), spare.contiguous(),
-                                                   parents.contiguous(), lengths.contiguous())
-        record("beam_reorder", dtype=str(k_cache.dtype), page=k_cache.shape[3])
-        return tuple(out)
     return reorder_reference(k_cache, v_cache, tables, spare, parents, lengths)
 
 

@@ -29,15 +29,18 @@ import torch
 
 from . import _native
 from .gated_reference import NEG_INF, work_dtype
-from .launch import record
+from .launch import count
 
-DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 MIN_PAGE = 16
 MAX_HEAD_DIM = 256
 
 
 def _check_cache(x, k_cache, v_cache, tables, positions):
-    """Checks shared by the two operators; ``x [batch, tokens, heads, head_dim]``."""
+    """Checks shared by the two operators; ``x [batch, tokens, heads, head_dim]``.
+
+    The extension makes the same ones (and that CUDA pools are contiguous and of
+    a native dtype) for CUDA tensors, where a call takes a few microseconds.
+    """
     if x.ndim != 4 or k_cache.ndim != 4 or k_cache.shape != v_cache.shape or x.shape[3] != k_cache.shape[3]:
         raise ValueError("expected rows [batch, tokens, heads, head_dim] and caches [pages, kv_heads, page, head_dim]")
     page, dim = k_cache.shape[2], k_cache.shape[3]
@@ -58,19 +61,6 @@ def _check_cache(x, k_cache, v_cache, tables, positions):
         raise ValueError("all tensors must be on one device")
     if torch.is_grad_enabled() and (x.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise ValueError("paged operators are for inference: they have no gradient")
-    if x.is_cuda:
-        if x.dtype not in DTYPES:
-            raise ValueError("the native paged operators take fp32, fp16 or bf16")
-        if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
-            raise ValueError("cache pools must be contiguous")
-
-
-def _int32(x):
-    return (x if x.dtype == torch.int32 else x.to(torch.int32)).contiguous()
-
-
-def _rows(x):
-    return x if x.stride(-1) == 1 else x.contiguous()
 
 
 def paged_append(q, k, v, cos, sin, k_cache, v_cache, tables, positions):
@@ -81,6 +71,10 @@ def paged_append(q, k, v, cos, sin, k_cache, v_cache, tables, positions):
     head_dim / 2]`` are fp32 (``RotaryEmbedding.tables``). The caches are
     updated in place; rows at position ``-1`` write nothing and give zeros.
     """
+    if q.is_cuda:
+        out = _native.native(q).paged_append(q, k, v, cos, sin, k_cache, v_cache, tables, positions)
+        count("paged_append", ("dtype", "head_dim", "page"), (q.dtype, q.shape[3], k_cache.shape[2]))
+        return out
     _check_cache(q, k_cache, v_cache, tables, positions)
     if k.shape != v.shape or k.shape != (*q.shape[:2], k_cache.shape[1], q.shape[3]):
         raise ValueError("expected k, v [batch, tokens, kv_heads, head_dim]")
@@ -91,11 +85,6 @@ def paged_append(q, k, v, cos, sin, k_cache, v_cache, tables, positions):
         raise ValueError("expected fp32 cos, sin [positions, head_dim / 2]")
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
         raise ValueError("paged operators are for inference: they have no gradient")
-    if q.is_cuda:
-        out = _native.native(q).paged_append(_rows(q), _rows(k), _rows(v), cos.contiguous(), sin.contiguous(),
-                                             k_cache, v_cache, tables.contiguous(), _int32(positions))
-        record("paged_append", dtype=str(q.dtype), head_dim=q.shape[3], page=k_cache.shape[2])
-        return out
     return append_reference(q, k, v, cos, sin, k_cache, v_cache, tables, positions)
 
 
@@ -104,13 +93,13 @@ def paged_attention(q, k_cache, v_cache, tables, positions):
 
     ``q [batch, tokens, heads, head_dim]``; the result has its shape and dtype.
     """
-    _check_cache(q, k_cache, v_cache, tables, positions)
     if q.is_cuda:
         ext = _native.native(q)
-        out = ext.paged_attention(q.contiguous(), k_cache, v_cache, tables.contiguous(), _int32(positions))
-        record("paged_attention", dtype=str(q.dtype), head_dim=q.shape[3], page=k_cache.shape[2],
-               path=ext.paged_attention_path(q, k_cache, v_cache))
+        out = ext.paged_attention(q, k_cache, v_cache, tables, positions)
+        count("paged_attention", ("dtype", "head_dim", "page", "path"),
+              (q.dtype, q.shape[3], k_cache.shape[2], ext.paged_attention_path(q, k_cache, v_cache)))
         return out
+    _check_cache(q, k_cache, v_cache, tables, positions)
     return attention_reference(q, k_cache, v_cache, tables, positions)
 
 

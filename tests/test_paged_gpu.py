@@ -331,3 +331,60 @@ def test_reorder_matches_definition(layers, groups, beams, kv, dim, page, length
     for mine, exact in zip((device[0], device[1], *got), (k, v, *want)):
         assert torch.equal(mine.cpu(), exact)
     assert torch.equal(device[2].cpu(), tables) and torch.equal(device[3].cpu(), spare)
+
+
+# ----------------------------------------------------------------------------
+# refusals
+# ----------------------------------------------------------------------------
+
+def test_native_refusals_are_the_same():
+    k, v, tables = make_cache([20], 2, 8, 16, torch.float32)
+    q, positions = torch.randn(1, 2, 4, 8, device="cuda"), torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+    new, cos = torch.randn(1, 2, 2, 8, device="cuda"), torch.zeros(20, 4, device="cuda")
+
+    def refuse(message, call, *args):
+        with pytest.raises(ValueError, match=message):
+            call(*args)
+
+    attend, append = paged.paged_attention, paged.paged_append
+    refuse("expected rows", attend, q[0], k, v, tables, positions)
+    refuse("expected rows", attend, q, k, v[:, :1], tables, positions)
+    refuse("power of two", attend, q, k[:, :, :8], v[:, :, :8], tables, positions)
+    refuse("head_dim", attend, q[..., :7], k[..., :7], v[..., :7], tables, positions)
+    refuse("multiple", attend, q[:, :, :3], k, v, tables, positions)
+    refuse("positions", attend, q, k, v, tables, positions[:, :1])
+    refuse("int32", attend, q, k, v, tables.long(), positions)
+    refuse("one dtype", attend, q.half(), k, v, tables, positions)
+    refuse("one device", attend, q, k, v, tables.cpu(), positions)
+    refuse("no gradient", attend, q.clone().requires_grad_(), k, v, tables, positions)
+    refuse("fp32, fp16 or bf16", attend, q.double(), k.double(), v.double(), tables, positions)
+    refuse("contiguous", attend, q, k.transpose(0, 1).contiguous().transpose(0, 1), v, tables, positions)
+    refuse("k, v", append, q, new[:, :1], new[:, :1], cos, cos, k, v, tables, positions)
+    refuse("match in dtype", append, q, new.half(), new.half(), cos, cos, k, v, tables, positions)
+    refuse("cos, sin", append, q, new, new, cos.double(), cos.double(), k, v, tables, positions)
+    logits, scores = torch.zeros(2, 3, 5, device="cuda"), torch.zeros(2, 3, device="cuda")
+    ended = torch.zeros(2, 3, dtype=torch.bool, device="cuda")
+    refuse("expected logits", beam.beam_select, logits[0], scores, ended, 0)
+    refuse("fp32", beam.beam_select, logits, scores.half(), ended, 0)
+    refuse("eos", beam.beam_select, logits, scores, ended, 5)
+    refuse("beams", beam.beam_select, torch.zeros(1, 33, 5, device="cuda"), torch.zeros(1, 33, device="cuda"),
+           torch.zeros(1, 33, dtype=torch.bool, device="cuda"), 0)
+    refuse("no gradient", beam.beam_select, logits.clone().requires_grad_(), scores, ended, 0)
+    pool = torch.zeros(1, 8, 1, 16, 2, device="cuda")
+    table, spare = torch.zeros(2, 3, 1, dtype=torch.int32, device="cuda"), torch.zeros(2, 3, dtype=torch.int32,
+                                                                                       device="cuda")
+    parents, lengths = spare.long(), torch.zeros(2, dtype=torch.int32, device="cuda")
+    refuse("expected pools", beam.beam_reorder, pool[0], pool[0], table, spare, parents, lengths)
+    refuse("int64", beam.beam_reorder, pool, pool, table, spare, parents.int(), lengths)
+    refuse("contiguous", beam.beam_reorder, pool.transpose(3, 4), pool.transpose(3, 4), table, spare, parents, lengths)
+
+
+def test_empty_calls():
+    k, v, tables = make_cache([20], 2, 64, 16, torch.bfloat16)
+    none = torch.zeros(1, 0, 4, 64, device="cuda", dtype=torch.bfloat16)
+    assert paged.paged_attention(none, k, v, tables, torch.zeros(1, 0, dtype=torch.int32, device="cuda")).numel() == 0
+    q = torch.ones(1, 2, 4, 64, device="cuda", dtype=torch.bfloat16)
+    hidden = torch.full((1, 2), -1, dtype=torch.int32, device="cuda")
+    assert not paged.paged_attention(q, k, v, tables, hidden).any()
+    assert not paged.paged_attention(q, k[:0], v[:0], tables, hidden).any()
+    assert not paged.paged_attention(q, k, v, tables[:, :0], hidden).any()
