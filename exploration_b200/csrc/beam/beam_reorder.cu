@@ -10,8 +10,8 @@
 // only, so no beam reads what another one writes and the CTAs need no order.
 //
 // Bound by memory: the filled rows of the copied pages, read and written once
-// with 16-byte vectors, four in flight a thread. One CTA takes one (beam, layer,
-// keys or values); the CTAs of the first layer also write the tables.
+// with 16-byte vectors, four in flight a thread. One CTA takes a few heads of one
+// (beam, layer, keys or values); the first one of a beam also writes its tables.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -33,7 +33,7 @@ struct ReorderArgs {
   int* tables_out;
   int* spare_out;
   int64_t layer_bytes, page_bytes, head_bytes;
-  int beams, width, pages, kv_heads, page, row_bytes;
+  int beams, width, pages, kv_heads, page, row_bytes, heads_per_cta;
 };
 
 template <typename V>
@@ -47,7 +47,7 @@ beam_reorder_kernel(ReorderArgs p) {
   const int* theirs = p.tables + static_cast<int64_t>(group * p.beams + parent) * p.width;
   const bool moves = parent != beam && rows > 0 && tail < p.width;
   const int fresh = p.spare[slot];
-  if (blockIdx.y == 0) {
+  if (blockIdx.y == 0 && blockIdx.z == 0) {
     int* out = p.tables_out + static_cast<int64_t>(slot) * p.width;
     for (int j = threadIdx.x; j < p.width; j += blockDim.x)
       out[j] = j < tail ? theirs[j] : (moves && j == tail ? fresh : mine[j]);
@@ -59,8 +59,12 @@ beam_reorder_kernel(ReorderArgs p) {
   char* cache = (blockIdx.y & 1 ? p.v : p.k) + (blockIdx.y >> 1) * p.layer_bytes;
   const char* src = cache + from * p.page_bytes;
   char* dst = cache + fresh * p.page_bytes;
+  // The heads of this CTA: each a contiguous span of `rows` rows.
+  const int h0 = blockIdx.z * p.heads_per_cta, heads = min(p.heads_per_cta, p.kv_heads - h0);
+  src += h0 * p.head_bytes;
+  dst += h0 * p.head_bytes;
   const int per_head = rows * (p.row_bytes / static_cast<int>(sizeof(V)));
-  const int total = per_head * p.kv_heads;
+  const int total = per_head * heads;
   auto place = [&](int i) {
     const int head = i / per_head;
     return head * p.head_bytes + static_cast<int64_t>(i - head * per_head) * sizeof(V);
@@ -69,16 +73,16 @@ beam_reorder_kernel(ReorderArgs p) {
   const int step = blockDim.x * kUnroll;
   for (int base = threadIdx.x; base < total; base += step) {
     V x[kUnroll];
+    int64_t at[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int i = base + u * blockDim.x;
-      if (i < total) x[u] = *reinterpret_cast<const V*>(src + place(i));
+      at[u] = i < total ? place(i) : -1;
+      if (at[u] >= 0) x[u] = *reinterpret_cast<const V*>(src + at[u]);
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int i = base + u * blockDim.x;
-      if (i < total) *reinterpret_cast<V*>(dst + place(i)) = x[u];
-    }
+    for (int u = 0; u < kUnroll; ++u)
+      if (at[u] >= 0) *reinterpret_cast<V*>(dst + at[u]) = x[u];
   }
 }
 
@@ -128,7 +132,9 @@ std::tuple<at::Tensor, at::Tensor> beam_reorder(at::Tensor& k_cache, at::Tensor&
   args.layer_bytes = args.pages * args.page_bytes;
   args.beams = spare.size(1);
   args.width = tables.size(2);
-  const dim3 grid(slots, std::max<int64_t>(1, 2 * layers));
+  // Heads of a CTA: about 16 KB of a full page, all of it in flight at once.
+  args.heads_per_cta = std::max<int64_t>(1, std::min<int64_t>(args.kv_heads, 16384 / args.head_bytes));
+  const dim3 grid(slots, std::max<int64_t>(1, 2 * layers), cdiv(args.kv_heads, args.heads_per_cta));
   auto stream = at::cuda::getCurrentCUDAStream();
   const bool wide = row_bytes % 16 == 0 && reinterpret_cast<uintptr_t>(args.k) % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(args.v) % 16 == 0;

@@ -4,12 +4,11 @@
 // lse_w = log sum_t exp(x_wt); an ended beam offers only (eos, c_w). Inside a
 // beam candidates are ordered by logit, then by token; across beams by score,
 // then by beam: rounding of the sum never reorders a beam's tokens, so each
-// beam's best `beams` logits are all that the final choice needs. A beam
-// whose lse is not finite (nothing left unmasked, or a NaN) offers -inf only.
+// beam's best `beams` logits are all that the final choice needs. A beam whose
+// lse is not finite (nothing left unmasked, or a NaN) offers tokens 0, 1, ... at -inf.
 //
 // Bound by one read of the logits (and by latency below a few MB). A warp holds
-// 1,024 logits in registers and takes its maximum, sum and best K from there:
-// per-lane bests, then K rounds of warp maximum / lowest index
+// 1,024 logits in registers and takes its maximum, sum and best K from there
 // (redux.sync on order-preserving integers). Up to 1,024 tokens one CTA a group
 // with a warp a beam does all in one launch. Longer rows are cut into chunks of
 // 8,192, one CTA each, whose sums and best K a second, overlapped launch joins:
@@ -32,6 +31,9 @@ constexpr int kWarpTokens = 32 * kPerLane;
 constexpr int kChunkWarps = 8;
 constexpr int kChunk = kChunkWarps * kWarpTokens;
 constexpr int kMaxBeams = 32;
+constexpr int kList = 64;           // candidates of a warp
+constexpr int kJoinWarps = 8;
+constexpr int kHeld = 8;            // candidates a lane of the joining warp holds
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct SelectArgs {
@@ -51,10 +53,35 @@ struct SelectArgs {
 // Order-preserving map of floats to unsigned integers.
 EB_DEVICE uint32_t ordered(float x) {
   const uint32_t u = __float_as_uint(x);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
 EB_DEVICE float unordered(uint32_t u) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+
+// Calls take(round, value, token) in every lane for the best `count` of the warp's
+// 64-bit keys (ordered value, inverted token; 0: none).
+template <int N, typename F>
+EB_DEVICE void pick_from(int count, uint64_t (&keys)[N], F take) {
+  for (int round = 0; round < count; ++round) {
+    uint64_t high = keys[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) high = keys[i] > high ? keys[i] : high;
+    const uint32_t value = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(high >> 32));
+    const uint32_t low = static_cast<uint32_t>(high >> 32) == value ? static_cast<uint32_t>(high) : 0u;
+    const uint32_t first = __reduce_max_sync(0xffffffffu, low);
+    take(round, unordered(value), value == 0 ? INT_MAX : static_cast<int>(0xffffffffu - first));
+    const uint64_t gone = static_cast<uint64_t>(value) << 32 | first;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (keys[i] == gone) keys[i] = 0;
+  }
+}
+
+template <typename F>
+EB_DEVICE void pick(int count, uint64_t a, uint64_t b, F take) {
+  uint64_t keys[2] = {a, b};
+  pick_from(count, keys, take);
 }
 
 // A lane's logits: kPerLane / VE vectors, vector j at index (j * 32 + lane) * VE of
@@ -78,57 +105,126 @@ struct LaneLogits {
         const uint4 u = *reinterpret_cast<const uint4*>(row + t);
         const T* h = reinterpret_cast<const T*>(&u);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) x[j * VE + i] = load_f<T>(h + i) + 0.f;   // -0 ties with 0
+        for (int i = 0; i < VE; ++i) x[j * VE + i] = load_f<T>(h + i);
       } else {
 #pragma unroll
         for (int i = 0; i < VE; ++i) 
-          x[j * VE + i] = t + i >= 0 && t + i < vocab ? load_f<T>(row + t + i) + 0.f : kNegInf;
+          x[j * VE + i] = t + i >= 0 && t + i < vocab ? load_f<T>(row + t + i) : kNegInf;
       }
     }
   }
 
-  // Maximum and sum of 2^((x - max) log2 e) over the warp.
-  EB_DEVICE void sum(float& m, float& s) const {
-    m = kNegInf;
+  // Maximum and sum of 2^((x - max) log2 e) over the warp; `peak`: of this lane alone.
+  EB_DEVICE void sum(float& m, float& s, float& peak) const {
+    peak = kNegInf;
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) m = fmaxf(m, x[i]);
-    m = warp_max(m);
-    const float ref = finite_or_zero(m);
-    s = 0.f;
+    for (int i = 0; i < kPerLane; ++i) peak = fmaxf(peak, x[i]);
+    m = warp_max(peak);
+    const float shift = finite_or_zero(m) * kLog2e;
+    float part[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) s += ex2((x[i] - ref) * kLog2e);
-    s = warp_sum(s);
+    for (int i = 0; i < kPerLane; ++i) part[i & 1] += ex2(fmaf(x[i], kLog2e, -shift));
+    s = warp_sum(part[0] + part[1]);
   }
 
-  // Calls take(round, value, token) in every lane for the best `count` logits in order.
+  // Bits of this lane's logits that exist.
+  EB_DEVICE uint32_t present(int vocab, int lane) const {
+    if (begin >= 0 && begin + kWarpTokens <= vocab) return 0xffffffffu;
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const int t = token(i, lane);
+      bits |= static_cast<uint32_t>(t >= 0 && t < vocab) << i;
+    }
+    return bits;
+  }
+
+  // Calls take(round, value, token) in every lane for the best `count` logits in order
+  // (token INT_MAX: no more). The count-th largest of the lanes' maxima bounds the
+  // count-th logit from below, so only the few logits that reach it are looked at
+  // further: they are read again and gathered into `list` (shared memory of this
+  // warp). Should few lanes hold too many of them, every round goes through all logits.
   template <typename F>
-  EB_DEVICE void best(int count, int vocab, int lane, F take) const {
-    uint32_t used = 0;
-    uint32_t key = 0;
-    int slot = 0;
-    auto rescan = [&]() {
-      key = 0;   // below every float's key
-      slot = -1;
+  EB_DEVICE void best(int count, int vocab, int lane, const T* row, float peak, uint64_t* list, F take) const {
+    const uint32_t valid = present(vocab, lane);
+    const uint32_t top = valid ? ordered(peak + 0.f) : 0u;   // -0 ties with 0; 0: below every float's key
+    uint32_t bound = top, left = top;
+    for (int round = 0; round < count; ++round) {
+      bound = __reduce_max_sync(0xffffffffu, left);
+      // One lane leaves the race; equal maxima count one by one.
+      if (lane == __ffs(__ballot_sync(0xffffffffu, left == bound)) - 1) left = 0;
+    }
+    bound = max(bound, ordered(kNegInf));
+    uint32_t above = 0, equal = 0;
+    if (top >= bound) {
+      const float limit = unordered(bound);
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) {
+        above |= static_cast<uint32_t>(x[i] > limit) << i;
+        equal |= static_cast<uint32_t>(x[i] == limit) << i;
+      }
+      above &= valid;
+      equal &= valid;
+    }
+    // Place of this lane's n entries among the warp's, and their total.
+    auto place = [&](int n, int& all) {
+      int upto = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      all = __shfl_sync(0xffffffffu, upto, 31);
+      return upto - n;
+    };
+    // Value first, then the lower token: one 64-bit key.
+    auto entry = [&](uint32_t k, int t) {
+      return static_cast<uint64_t>(k) << 32 | (0xffffffffu - static_cast<uint32_t>(t));
+    };
+    int total;
+    int at = place(__popc(above), total);
+    if (total + count <= kList) {
+      for (; above; above &= above - 1) {
+        const int t = token(__ffs(above) - 1, lane);
+        list[at++] = entry(ordered(load_f<T>(row + t) + 0.f), t);
+      }
+      // Of the logits equal to the bound (all of a masked stretch, perhaps) the first `count` tokens.
+      const int limit = total + count;
+#pragma unroll 1
+      for (int j = 0; j < kPerLane / VE && total < limit; ++j) {
+        uint32_t mine = equal >> (j * VE) & ((1u << VE) - 1);
+        if (!__any_sync(0xffffffffu, mine != 0)) continue;
+        int all;
+        int slot = total + place(__popc(mine), all);
+        for (; mine && slot < limit; mine &= mine - 1) list[slot++] = entry(bound, token(j * VE + __ffs(mine) - 1, lane));
+        total += all;
+      }
+      total = min(total, limit);
+      __syncwarp();
+      pick(count, lane < total ? list[lane] : 0, lane + 32 < total ? list[lane + 32] : 0, take);
+      __syncwarp();
+      return;
+    }
+    uint32_t last_key = 0xffffffffu;
+    int last_token = -1;
+    for (int round = 0; round < count; ++round) {
+      uint32_t key = 0;
+      int t_best = INT_MAX;
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i) {
         const int t = token(i, lane);
-        const uint32_t k = ordered(x[i]);
-        if (!(used >> i & 1) && t >= 0 && t < vocab && (slot < 0 || k > key)) {
+        const uint32_t k = ordered(x[i] + 0.f);
+        const bool after = k < last_key || (k == last_key && t > last_token);   // not taken yet
+        if ((valid >> i & 1) && after && (t_best == INT_MAX || k > key)) {
           key = k;
-          slot = i;
+          t_best = t;
         }
       }
-    };
-    rescan();
-    for (int round = 0; round < count; ++round) {
-      const uint32_t top = __reduce_max_sync(0xffffffffu, slot < 0 ? 0u : key);
-      const int mine = slot >= 0 && key == top ? token(slot, lane) : INT_MAX;
-      const int first = __reduce_min_sync(0xffffffffu, mine);
-      take(round, unordered(top), first);
-      if (mine == first && first != INT_MAX) {
-        used |= 1u << slot;
-        rescan();
-      }
+      const uint32_t value = __reduce_max_sync(0xffffffffu, t_best == INT_MAX ? 0u : key);
+      const int first = __reduce_min_sync(0xffffffffu, t_best != INT_MAX && key == value ? t_best : INT_MAX);
+      take(round, unordered(value), first);
+      last_key = value;
+      last_token = first;
     }
   }
 };
@@ -168,9 +264,12 @@ EB_DEVICE void offer(const SelectArgs& p, int row, float lse, int i, float x, in
   if (p.finished[row]) {
     total = i == 0 ? base : kNegInf;
     token = p.eos;
+  } else if (!isfinite(lse)) {
+    total = kNegInf;
+    token = i;
   } else {
     const float sum = __fadd_rn(base, __fsub_rn(x, lse));
-    total = isfinite(lse) && sum == sum ? sum : kNegInf;
+    total = sum == sum ? sum : kNegInf;
     token = t;
   }
 }
@@ -181,16 +280,17 @@ __global__ void __launch_bounds__(1024)
 beam_select_small_kernel(SelectArgs p) {
   __shared__ float total[kMaxBeams][kMaxBeams];
   __shared__ int token[kMaxBeams][kMaxBeams];
+  __shared__ uint64_t list[kMaxBeams][kList];
   const int group = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = group * p.beams + warp;
   {
     const T* logits = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.vocab;
     LaneLogits<T> x;
     x.load(logits, aligned_start(logits), p.vocab, lane);
-    float m, s;
-    x.sum(m, s);
+    float m, s, peak;
+    x.sum(m, s, peak);
     const float lse = m + logf(s);
-    x.best(p.keep, p.vocab, lane, [&](int i, float value, int t) {
+    x.best(p.keep, p.vocab, lane, logits, peak, list[warp], [&](int i, float value, int t) {
       if (lane == 0) offer(p, row, lse, i, value, t, total[warp][i], token[warp][i]);
     });
   }
@@ -200,23 +300,25 @@ beam_select_small_kernel(SelectArgs p) {
 
 // Longer rows, first launch: sums and best K of one chunk.
 template <typename T>
-__global__ void __launch_bounds__(kChunkWarps * 32)
+__global__ void __launch_bounds__(kChunkWarps * 32, 3)
 beam_select_chunk_kernel(SelectArgs p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the joining CTAs may be set up
   __shared__ float sm_m[kChunkWarps], sm_s[kChunkWarps];
   __shared__ float sm_x[kChunkWarps][kMaxBeams];
   __shared__ int sm_t[kChunkWarps][kMaxBeams];
+  __shared__ uint64_t list[kChunkWarps][kList];
   const int chunk = blockIdx.x, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T* logits = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.vocab;
   {
     LaneLogits<T> x;
     x.load(logits, aligned_start(logits) + static_cast<int64_t>(chunk) * kChunk + warp * kWarpTokens, p.vocab, lane);
-    float m, s;
-    x.sum(m, s);
+    float m, s, peak;
+    x.sum(m, s, peak);
     if (lane == 0) {
       sm_m[warp] = m;
       sm_s[warp] = s;
     }
-    x.best(p.keep, p.vocab, lane, [&](int i, float value, int t) {
+    x.best(p.keep, p.vocab, lane, logits, peak, list[warp], [&](int i, float value, int t) {
       if (lane == 0) {
         sm_x[warp][i] = value;
         sm_t[warp][i] = t;
@@ -253,28 +355,42 @@ beam_select_chunk_kernel(SelectArgs p) {
   }
 }
 
-// Second launch: one CTA a group, one warp a beam joins its chunks, then the choice.
-__global__ void __launch_bounds__(1024)
-beam_select_join_kernel(SelectArgs p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  __shared__ float total[kMaxBeams][kMaxBeams];
-  __shared__ int token[kMaxBeams][kMaxBeams];
-  const int group = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = group * p.beams + warp;
+// One warp: a beam's sums and best logits from its chunks'.
+EB_DEVICE void join_beam(const SelectArgs& p, int row, int lane, float* total, int* token) {
   const int64_t base = static_cast<int64_t>(row) * p.chunks;
   float m = kNegInf;
   for (int c = lane; c < p.chunks; c += 32) m = fmaxf(m, p.part_ms[(base + c) * 2]);
   m = warp_max(m);
   const float ref = finite_or_zero(m);
+  // The chunks' sums are added in fp64: lse depends on the cut by no more than its own rounding.
   double sum = 0.0;
   for (int c = lane; c < p.chunks; c += 32) {
     const float2 ms = *reinterpret_cast<const float2*>(p.part_ms + (base + c) * 2);
-    sum += static_cast<double>(ms.y) * exp(static_cast<double>(ms.x) - ref);
+    sum += static_cast<double>(ms.y * ex2((ms.x - ref) * kLog2e));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float lse = static_cast<float>(static_cast<double>(m) + log(sum));
-  // K rounds over the chunks' sorted lists: chunk c belongs to lane c % 32.
+  const float lse = m + logf(static_cast<float>(sum));
+  const int entries = p.chunks * p.keep;
+  if (entries <= 32 * kHeld) {
+    uint64_t keys[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int e = i * 32 + lane;
+      keys[i] = 0;
+      if (e < entries) {
+        const int t = p.part_t[base * p.keep + e];
+        if (t != INT_MAX)
+          keys[i] = static_cast<uint64_t>(ordered(p.part_x[base * p.keep + e])) << 32 |
+                    (0xffffffffu - static_cast<uint32_t>(t));
+      }
+    }
+    pick_from(p.keep, keys, [&](int i, float value, int t) {
+      if (lane == 0) offer(p, row, lse, i, value, t, total[i], token[i]);
+    });
+    return;
+  }
+  // Longer: K rounds over the chunks' sorted lists, chunk c with lane c % 32.
   uint32_t key = 0;
   int mine = INT_MAX;
   // A lane with several chunks rescans their lists for its best entry after (last value, last token).
@@ -302,15 +418,26 @@ beam_select_join_kernel(SelectArgs p) {
     const uint32_t top = __reduce_max_sync(0xffffffffu, mine == INT_MAX ? 0u : key);
     const int cand = mine != INT_MAX && key == top ? mine : INT_MAX;
     const int first = __reduce_min_sync(0xffffffffu, cand);
-    if (lane == 0) offer(p, row, lse, round, unordered(top), first, total[warp][round], token[warp][round]);
+    if (lane == 0) offer(p, row, lse, round, unordered(top), first, total[round], token[round]);
     if (cand == first && first != INT_MAX) {
       last_key = key;
       last_t = mine;
       rescan();
     }
   }
+}
+
+// Second launch: one CTA a group; warps take the beams in turn and join their chunks, then the choice.
+__global__ void __launch_bounds__(kJoinWarps * 32)
+beam_select_join_kernel(SelectArgs p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ float total[kMaxBeams][kMaxBeams];
+  __shared__ int token[kMaxBeams][kMaxBeams];
+  const int group = blockIdx.x, lane = threadIdx.x & 31;
+  for (int beam = threadIdx.x >> 5; beam < p.beams; beam += blockDim.x >> 5)
+    join_beam(p, group * p.beams + beam, lane, total[beam], token[beam]);
   __syncthreads();
-  if (warp == 0) choose(p, group, lane, total, token);
+  if (threadIdx.x < 32) choose(p, group, lane, total, token);
 }
 
 template <typename T>
@@ -332,7 +459,7 @@ void launch(SelectArgs& args, int groups, const at::TensorOptions& f32, cudaStre
   EB_CUDA_CHECK(cudaGetLastError());
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(groups);
-  config.blockDim = dim3(32 * args.beams);
+  config.blockDim = dim3(32 * std::min(args.beams, kJoinWarps));
   config.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

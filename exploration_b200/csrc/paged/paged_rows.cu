@@ -37,11 +37,12 @@ constexpr int kWholeTiles = 16;   // items of up to 1,024 keys are not cut: join
 constexpr int kConsumers = 4;
 constexpr int kThreads = 32 * (kConsumers + 1);
 
+// CTAs an SM and stages of each, within shared memory and registers.
 template <int D>
 struct RowsConfig;
 template <>
 struct RowsConfig<64> {
-  static constexpr int kStages = 5, kCtas = 2;
+  static constexpr int kStages = 3, kCtas = 3;
 };
 template <>
 struct RowsConfig<128> {
@@ -113,25 +114,26 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         }
         const int key0 = tile * kTile;
         const int boxes = min(pages_tile, cdiv(s.limit - key0, box));
+        // Lane i fetches box i (at most four a tile). An entry outside the pool reads as
+        // zeros (out of the map's bounds), never foreign memory.
+        if ((key0 >> p.page_shift) - base >= 32) {
+          base += 32;
+          ids = ahead;
+          ahead = entry(base + 32 + lane);
+        }
+        const int want = ((key0 + min(lane, boxes - 1) * box) >> p.page_shift) - base;
+        const int id_low = __shfl_sync(0xffffffffu, ids, want & 31), id_high = __shfl_sync(0xffffffffu, ahead, want & 31);
+        const int id = want < 32 ? id_low : id_high;
+        const int plane = id >= 0 && id < p.pages ? id * p.kv_heads + kv_head : p.pages * p.kv_heads;
         if (lane == 0) mbar_expect_tx(&sm.full[stage], boxes * box * D * 2 * 2);
-        for (int i = 0; i < boxes; ++i) {
-          const int key = key0 + i * box, page = key >> p.page_shift;
-          if (page - base >= 32) {
-            base += 32;
-            ids = ahead;
-            ahead = entry(base + 32 + lane);
-          }
-          // An entry outside the pool loads zeros (out of the map's bounds), never foreign memory.
-          const int id = __shfl_sync(0xffffffffu, ids, page - base);
-          const int plane = id >= 0 && id < p.pages ? id * p.kv_heads + kv_head : p.pages * p.kv_heads;
-          if (lane == 0) {
+        __syncwarp();
+        if (lane < boxes) {
 #pragma unroll
-            for (int h = 0; h < D / 64; ++h) {
-              tma_load_3d(&sm.kv[stage][0][h * kHalf + i * box * 64], &tk, &sm.full[stage], h * 64,
-                          key & (p.page - 1), plane);
-              tma_load_3d(&sm.kv[stage][1][h * kHalf + i * box * 64], &tv, &sm.full[stage], h * 64,
-                          key & (p.page - 1), plane);
-            }
+          for (int h = 0; h < D / 64; ++h) {
+            tma_load_3d(&sm.kv[stage][0][h * kHalf + lane * box * 64], &tk, &sm.full[stage], h * 64,
+                        (key0 + lane * box) & (p.page - 1), plane);
+            tma_load_3d(&sm.kv[stage][1][h * kHalf + lane * box * 64], &tv, &sm.full[stage], h * 64,
+                        (key0 + lane * box) & (p.page - 1), plane);
           }
         }
         ++issued;

@@ -33,6 +33,7 @@ from torch.utils.checkpoint import checkpoint
 
 from ..ops import fused
 from ..ops.flash import flash_attention
+from ..ops.paged import paged_append, paged_attention
 from ..parallel.context import ParallelContext
 from .blocks import FeedForward, RotaryEmbedding
 from .head import sliced_head_loss
@@ -84,6 +85,15 @@ class BaselineBlock(nn.Module):
         y = fused.linear_residual(self.context(x, positions, parallel), self.out, x)
         return fused.ffn_residual(fused.layer_norm(y, self.ffn_norm), y, self.ffn)
 
+    def decode(self, x, k_cache, v_cache, cos, sin, tables, positions):
+        """New tokens ``x [B, n, D]`` over (and into) this layer's paged cache."""
+        batch, n, dim = x.shape
+        qkv = fused.linear(fused.layer_norm(x, self.attn_norm), self.qkv).view(batch, n, 3, self.heads, self.hd)
+        q = paged_append(*qkv.unbind(2), cos, sin, k_cache, v_cache, tables, positions)
+        ctx = paged_attention(q, k_cache, v_cache, tables, positions).reshape(batch, n, dim)
+        y = fused.linear_residual(ctx, self.out, x)
+        return fused.ffn_residual(fused.layer_norm(y, self.ffn_norm), y, self.ffn)
+
     def forward(self, x, positions, parallel=None, checkpoint_chunks=False):
         parallel = parallel or ParallelContext()
         if checkpoint_chunks and torch.is_grad_enabled():
@@ -122,6 +132,21 @@ class BaselineModel(nn.Module):
         for block in self.blocks:
             x = block(x, positions, parallel, self.checkpoint_chunks)
         return x
+
+    def decode(self, input_ids, k_cache, v_cache, cos, sin, tables, positions):
+        """Residual stream of new tokens ``[B, n]`` over a paged cache (inference; see ops/paged.py).
+
+        ``k_cache, v_cache [layers, pages, heads, page, head_dim]`` share one set of ``tables``; ``cos, sin``
+        are the rotation's fp32 tables. The cache is extended in place.
+        """
+        x = self.embedding(input_ids)
+        for i, block in enumerate(self.blocks):
+            x = block.decode(x, k_cache[i], v_cache[i], cos, sin, tables, positions)
+        return x
+
+    def logits(self, x):
+        """Logits of residual-stream rows ``x [..., D]``."""
+        return self._logits(x)
 
     def _logits(self, x):
         return fused.linear(fused.layer_norm(x, self.final_norm), self.lm_head)

@@ -31,7 +31,7 @@ def beam_select(logits, scores, finished, eos):
     token ``t`` at ``score + (logit_t - logsumexp(logits))``; a finished one
     offers only ``(eos, score)``. Candidates are ordered inside a beam by logit,
     then token, and across beams by score (fp32), then beam, best first. A
-    beam whose logsumexp is not finite offers ``-inf``. ``parents`` and
+    beam whose logsumexp is not finite offers tokens ``0, 1, ...`` at ``-inf``. ``parents`` and
     ``tokens`` are int64; ``finished`` is true for an ended parent or token
     ``eos`` (``-1``: no token ends a beam).
     """
@@ -98,8 +98,10 @@ def select_reference(logits, scores, finished, eos):
     best, token = x.sort(dim=-1, descending=True, stable=True)
     best, token = best[..., :keep], token[..., :keep]
     total = scores[..., None] + (best - lse).float()
+    rank = torch.arange(keep, device=logits.device)
     total = torch.where(torch.isfinite(lse) & ~total.isnan(), total, NEG_INF)
-    first = torch.arange(keep, device=logits.device) == 0
+    token = torch.where(torch.isfinite(lse), token, rank)
+    first = rank == 0
     ended = finished[..., None]
     total = torch.where(ended, torch.where(first, scores[..., None], NEG_INF), total)
     token = torch.where(ended, eos, token)

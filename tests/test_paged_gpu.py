@@ -311,6 +311,23 @@ def test_select_masked_and_dead_beams(vocab):
     check_select(logits, scores, finished, eos=4)
 
 
+@pytest.mark.parametrize("vocab", [50, 9000])
+def test_select_all_beams_dead(vocab):
+    logits = torch.full((2, 3, vocab), -math.inf)
+    logits[1, :, 4] = math.nan
+    check_select(logits, torch.zeros(2, 3), torch.zeros(2, 3, dtype=torch.bool), eos=1)
+
+
+@pytest.mark.parametrize("vocab", [900, 30000])
+def test_select_best_tokens_side_by_side(vocab):
+    """Many of the best logits in few lanes, in rising, falling and equal runs."""
+    logits = torch.randn(3, 8, vocab, generator=torch.Generator().manual_seed(2))
+    logits[0, :, 100:300] = torch.linspace(9, 12, 200)
+    logits[1, :, 100:300] = torch.linspace(12, 9, 200)
+    logits[2, :, 64:320] = 10.0
+    check_select(logits, -torch.rand(3, 8).cumsum(1), torch.zeros(3, 8, dtype=torch.bool), eos=-1)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("layers,groups,beams,kv,dim,page,lengths", [
     (1, 1, 1, 1, 64, 16, [5]), (2, 3, 4, 2, 64, 16, [1, 16, 31]), (3, 2, 6, 4, 64, 32, [63, 64]),
