@@ -41,6 +41,7 @@ SOURCES = [
     "paged/paged_simt.cu",
     "paged/paged_rows.cu",
     "paged/paged_chunk_tc.cu",
+    "paged/paged_tile_fp32.cu",
     "paged/paged_combine.cu",
     "beam/beam_select.cu",
     "beam/beam_reorder.cu",

@@ -128,5 +128,6 @@ template <typename T>
 void paged_rows_launch(paged::Args& args, int sms, cudaStream_t stream);
 template <typename T>
 void paged_chunk_launch(paged::Args& args, int sms, cudaStream_t stream);
+void paged_tile_fp32_launch(paged::Args& args, int sms, cudaStream_t stream);
 
 }  // namespace eb
