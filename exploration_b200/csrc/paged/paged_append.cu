@@ -10,6 +10,9 @@
 // a token's rotation row are shared by all heads through L1. One CTA takes one
 // token, so position, page and rotation row are looked up once; a thread takes
 // one 16-byte vector of the first half of a head and its partner in the second.
+// Measured: 4,245 tokens in 4 x 2,011 rows, 32 + 2 x 8 heads of 128, bf16 (138 MB): 25.5 us of
+// kernel, 5.4 TB/s. CTAs of 384 threads (a vector pair each, 33 us) and loads begun
+// before the position is known (32.6 us) were slower.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

@@ -26,6 +26,19 @@
 //
 // TMEM columns: score buffers from 0, then the two accumulators of D columns.
 //
+// Measured: 2,048 tokens over 65,536 keys, 16 heads of 64, bf16: 0.64 ms in a short
+// burst (850 TFLOP/s), 0.76 ms sustained under the power cap (713); ragged chunks of
+// 1,111 tokens over up to 8,191 keys, 32/8 heads of 128, fp16: 0.42 and 0.47 ms (721).
+// At head dim 64 a step is bound by the softmax instructions of two warps an SM
+// sub-partition (their special-function share alone is 2,048 cycles of 2,500) and the
+// hand-overs around them; at 128 by the chain weights -> P V -> next S -> softmax
+// (3,300 cycles for 2,056 of tensor work). A finished barrier costs a waiting warp some
+// 90 cycles, so what did not pay: exponentials on the FMA pipe, two issuing threads,
+// scores released early, strict turns of the warpgroups, shorter steps.
+//
+// Non-finite values of a key that some row of the call sees may reach its other
+// rows: a weight of zero times a NaN is a NaN in the matrix unit.
+//
 // Keys past an item's limit are masked, and their V rows cleared: a page's
 // unwritten rows may hold anything.
 #include <ATen/ATen.h>

@@ -12,6 +12,12 @@
 // round trip through tensor memory (and without padding 16 rows to 128) that
 // tcgen05 would cost here; arithmetic hides under the loads.
 //
+// Measured: one token of 64 sequences of 17 to 16,384 keys, 32/8 heads of 128,
+// bf16 (2.15 GB): 0.352 ms, 6.1 TB/s, 93% of the measured copy bandwidth. Five
+// tokens of 16 sequences of up to 4,099 keys, 16 heads of 64, fp16 (148 MB): 31.4 us
+// of kernel, bound by its start (positions, tables, first tiles: 4.5 us) and by the
+// joining launch after it (5 us).
+//
 // Keys past an item's limit are masked, their values cleared in the fragments:
 // a page's unwritten rows may hold anything.
 #include <ATen/ATen.h>
@@ -33,11 +39,14 @@ using namespace sm100;
 
 constexpr int kRows = 16;
 constexpr int kTile = 64;
-constexpr int kWholeTiles = 16;   // items of up to 1,024 keys are not cut: joining costs a launch
+// Items of up to 1,024 keys are not cut, because joining costs a launch: 4 sequences of
+// up to 517 keys, 4 heads of 64, take one kernel of 8.1 us whole, 5.3 + 3.5 us cut.
+constexpr int kWholeTiles = 16;
 constexpr int kConsumers = 4;
 constexpr int kThreads = 32 * (kConsumers + 1);
 
-// CTAs an SM and stages of each, within shared memory and registers.
+// CTAs an SM and stages of each, within shared memory and registers (head dim 64: three
+// CTAs of three stages 38.1 us for the drafted tokens above, two of five 39.0 us).
 template <int D>
 struct RowsConfig;
 template <>

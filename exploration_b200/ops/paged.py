@@ -16,7 +16,8 @@ one captured CUDA graph of a step serves every later step.
 Both are for inference: they have no gradient and refuse inputs that need
 one. CUDA tensors (fp32, fp16, bf16) run the sm_100a kernels of
 ``csrc/paged``; CPU tensors run the definitions below. Rows of the cache past
-a sequence's largest position may hold anything. A position past the end of
+a sequence's largest position may hold anything (a non-finite key or value that
+one row of a call sees may reach the call's other rows of that sequence). A position past the end of
 the table (or of the rotation tables) or a table entry outside the pool is
 the caller's error: CUDA kernels stay inside the buffers, what such rows
 read or lose is undefined.
