@@ -59,6 +59,7 @@ using namespace paged;
 using namespace sm100;
 
 constexpr int kM = 128;               // rows of an MMA
+constexpr int kItemCost = 3;   // of an item's start and end, in tiles
 constexpr int kTile = 128;            // keys of a tile
 constexpr int kBox = 128 * 64;        // elements of a 64-wide half of a 128-row operand
 constexpr int kThreads = 384;
@@ -69,12 +70,15 @@ template <int D>
 struct alignas(1024) ChunkSmem {
   static constexpr int kStages = D == 64 ? 4 : 2;   // of each ring
   static constexpr int kBufs = (kTmemCols - 2 * D) / 128;   // score buffers in TMEM
+  // With two buffers the next scores wait for this step's products: those of the
+  // first half of the keys begin while the second half's weights are computed.
+  static constexpr bool kHalves = kBufs == 2;
   uint16_t q[2][kM * D];
   uint16_t k[kStages][kTile * D];
   uint16_t v[kStages][kTile * D];
   uint64_t q_full, q_empty;
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[kBufs], p_full[kBufs], o_done[2], join, v_ragged, v_clear;
+  uint64_t s_full[kBufs], p_full[kBufs], p_half[kBufs], o_done[2], join, v_ragged, v_clear;
   uint32_t tmem_base;
   int abort;
   int clear_stage;
@@ -142,6 +146,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   ChunkSmem<D>& sm = *reinterpret_cast<ChunkSmem<D>*>(
       (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
   constexpr int kStages = ChunkSmem<D>::kStages, kBufs = ChunkSmem<D>::kBufs;
+  constexpr bool kHalves = ChunkSmem<D>::kHalves;
   constexpr int kO = kTmemCols - 2 * D;          // first TMEM column of the accumulators
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort = &sm.abort;
@@ -157,6 +162,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     for (int b = 0; b < kBufs; ++b) {
       mbar_init(&sm.s_full[b], 1);
       mbar_init(&sm.p_full[b], 128);
+      mbar_init(&sm.p_half[b], 128);
     }
     mbar_init(&sm.o_done[0], 1);
     mbar_init(&sm.o_done[1], 1);
@@ -313,14 +319,21 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
               ok = wait_tight(&sm.v_clear, clear_phase, abort, err, kSiteKvFull);
             }
           }
-          ok = ok && wait_tight(&sm.p_full[pr.stage], pr.phase, abort, err, kSitePFull);
+          ok = ok && wait_tight(kHalves ? &sm.p_half[pr.stage] : &sm.p_full[pr.stage], pr.phase, abort, err, kSitePFull);
           if (!ok) break;
           tc_fence_after();
           const uint32_t v_lo = desc_lo(sm.v[vr.stage], kBox * 2);
           const uint32_t o_addr = tmem + kO + w * D, p_addr = tmem + pr.stage * 128, more = i > 1;
 #pragma unroll
-          for (int kk = 0; kk < kTile / 16; ++kk)
+          for (int kk = 0; kk < kTile / 16; ++kk) {
+            if (kHalves && kk == kTile / 32) {
+              ok = wait_tight(&sm.p_full[pr.stage], pr.phase, abort, err, kSitePFull);
+              if (!ok) break;
+              tc_fence_after();
+            }
             mma_ts_lo<kDescHi>(o_addr, p_addr + kk * 8, v_lo + kk * (2048 >> 4), id_pv, kk > 0 ? 1u : more);
+          }
+          if (!ok) break;
           tc_commit(&sm.o_done[w]);
           pr.next(kBufs);
           if (!dual || w == 1) {
@@ -456,6 +469,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             packed[i] = pack2<T>(e.x, e.y);   // weights rounded for the second product, their sum is not
           }
           tmem_st16(s_addr + c / 2, packed);
+          if (kHalves && c == kTile / 2 - 32) {
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(&sm.p_half[buf]);
+          }
         }
         sum[0] = add2(sum[0], sum[1]);
         l = l * alpha + (sum[0].x + sum[0].y);
@@ -551,7 +569,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
 
 template <typename T, int D>
 void launch(Args& args, int sms, cudaStream_t stream) {
-  const Split split(args, sms, 0);
+  const Split split(args, sms, 0, kItemCost);
   constexpr bool kHalf = std::is_same_v<T, __half>;
   const CUtensorMap tq = make_query_map(args, kHalf, kM / args.group);
   const CUtensorMap tk = make_pool_map(args, args.k, kHalf, kTile);

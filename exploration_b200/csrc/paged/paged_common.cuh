@@ -14,7 +14,9 @@
 // the device) says how long a sequence is: one captured launch serves every
 // later step. The key tiles of all (entry, key head) items form one list, cut
 // into equal runs, one a CTA: sequences of very different lengths and a few
-// rows over a long cache both fill the GPU. An item inside one run is written
+// rows over a long cache both fill the GPU. Each item counts a few tiles more, for
+// its start and end (with tiles alone the CTA that got fifteen short items of a
+// ragged chunk took 409 us, most others 340). An item inside one run is written
 // out by its CTA; an item that is cut leaves unnormalised partial sums (at most
 // two a CTA: its first and its last item), which the combine kernel joins in
 // key order, so results do not depend on the order in which CTAs finish. Each
@@ -39,7 +41,7 @@ struct Args {
   float* part_o;          // [2 * CTAs, row_tile, dim] partial sums of 2^(a - m) v
   float* part_ml;         // [2 * CTAs, row_tile, 2]: m (base 2), sum of 2^(a - m)
   int* cuts;              // [CTAs, 4]: entry, head, first tile and tiles of the item that a CTA's run begins in
-  int* run;               // [1] tiles of a run
+  int* run;               // [1] units of a run
   int batch, tokens, heads, kv_heads, dim;
   int group;              // query heads of an item
   int item_heads;         // items of an entry: kv_heads, or a multiple when an item takes part of a head's group
@@ -50,7 +52,7 @@ struct Args {
   int row_tiles;          // row tiles of a sequence
   int key_tile;           // keys of a tile
   int flat;               // 1: equal runs of the tile list; 0: one item a CTA (too many entries for the table)
-  int min_run;            // fewest tiles of a run
+  int item_cost;          // what starting and finishing an item costs, in tiles of work
   float scale_log2;       // log2(e) / sqrt(dim)
 };
 
@@ -83,17 +85,20 @@ EB_DEVICE int entry_limit_warp(const Args& p, int entry, int lane) {
   return static_cast<int>(min(static_cast<int64_t>(top) + 1, static_cast<int64_t>(p.width) * p.page));
 }
 
-// Prefix of the entries' key tiles into cum[0 .. entries] (shared memory); all threads.
+// Units of an item of `limit` keys: its tiles, then its fixed cost.
+EB_DEVICE int entry_units(const Args& p, int limit) { return limit > 0 ? cdiv(limit, p.key_tile) + p.item_cost : 0; }
+
+// Prefix of the entries' units into cum[0 .. entries] (shared memory); all threads.
 EB_DEVICE void build_prefix(const Args& p, int* cum) {
   const int entries = p.batch * p.row_tiles;
   if (p.tile_tokens <= 16) {
     for (int e = threadIdx.x; e < entries; e += blockDim.x)
-      cum[e + 1] = cdiv(entry_limit(p, e), p.key_tile);
+      cum[e + 1] = entry_units(p, entry_limit(p, e));
   } else {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int e = warp; e < entries; e += blockDim.x >> 5) {
       const int n = entry_limit_warp(p, e, lane);
-      if (lane == 0) cum[e + 1] = cdiv(n, p.key_tile);
+      if (lane == 0) cum[e + 1] = entry_units(p, n);
     }
   }
   if (threadIdx.x == 0) cum[0] = 0;
@@ -116,27 +121,26 @@ EB_DEVICE void build_prefix(const Args& p, int* cum) {
   __syncthreads();
 }
 
-// Tiles of one run.
-EB_DEVICE int64_t run_tiles(const Args& p, int total, int ctas) {
-  const int64_t all = static_cast<int64_t>(total) * p.item_heads;
-  const int64_t run = (all + ctas - 1) / ctas;
-  return run < p.min_run ? p.min_run : run;
+// Units of one run (all of a call's units fit an int: see the launch).
+EB_DEVICE int run_units(const Args& p, int total, int ctas) {
+  const int all = total * p.item_heads;
+  return all / ctas + (all % ctas != 0);
 }
 
 // Walks the segments of one CTA's run. `cum` is unused when flat == 0.
 struct Walk {
-  int64_t at, end, first;
+  int at, end, first;
   int entry_hint;
 
   EB_DEVICE void start(const Args& p, const int* cum) {
     if (p.flat) {
       const int total = cum[p.batch * p.row_tiles];
-      const int64_t run = run_tiles(p, total, gridDim.x), all = static_cast<int64_t>(total) * p.item_heads;
-      at = static_cast<int64_t>(blockIdx.x) * run;
-      end = at + run < all ? at + run : all;
+      const int run = run_units(p, total, gridDim.x), all = total * p.item_heads;
+      at = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * run, static_cast<int64_t>(all)));
+      end = all - at < run ? all : at + run;
     } else {
       // Latest row tiles first: they hold the most keys of a causal chunk.
-      at = static_cast<int64_t>(p.batch) * p.row_tiles * p.item_heads - 1 - blockIdx.x;
+      at = p.batch * p.row_tiles * p.item_heads - 1 - static_cast<int>(blockIdx.x);
       end = at + 1;
     }
     first = at;
@@ -146,34 +150,39 @@ struct Walk {
   // The next segment, or false. Uniform over the threads that call it. In the
   // one-item form the segment may be empty (begin == end, slot -1): the output is zero.
   EB_DEVICE bool next(const Args& p, const int* cum, Segment& s) {
-    if (at >= end) return false;
-    int tiles;
-    if (p.flat) {
-      const int entries = p.batch * p.row_tiles;
-      int lo = entry_hint, hi = entries;
-      while (hi - lo > 1) {   // last entry whose items start at or before `at` (never an empty one)
-        const int mid = (lo + hi) >> 1;
-        if (static_cast<int64_t>(cum[mid]) * p.item_heads <= at) lo = mid;
-        else hi = mid;
+    while (true) {
+      if (at >= end) return false;
+      const int here = at;
+      if (!p.flat) {
+        s.entry = at / p.item_heads;
+        s.head = at - s.entry * p.item_heads;
+        s.slot = -1;
+        ++at;
+      } else {
+        const int entries = p.batch * p.row_tiles;
+        int lo = entry_hint, hi = entries;
+        while (hi - lo > 1) {   // last entry whose items start at or before `at` (never an empty one)
+          const int mid = (lo + hi) >> 1;
+          if (cum[mid] * p.item_heads <= at) lo = mid;
+          else hi = mid;
+        }
+        s.entry = lo;
+        entry_hint = lo;
+        const int units = cum[lo + 1] - cum[lo], tiles = units - p.item_cost;
+        const int rel = at - cum[lo] * p.item_heads;
+        s.head = rel / units;
+        const int unit = rel - s.head * units;
+        const int n = min(units - unit, end - at);
+        s.begin = min(unit, tiles);
+        s.end = min(unit + n, tiles);
+        at += n;
+        if (s.begin == s.end) continue;   // only the item's fixed cost fell into this run
+        s.slot = s.begin == 0 && s.end == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (here == first ? 0 : 1);
       }
-      s.entry = lo;
-      entry_hint = lo;
-      tiles = cum[lo + 1] - cum[lo];
-      const int64_t rel = at - static_cast<int64_t>(cum[lo]) * p.item_heads;
-      s.head = static_cast<int>(rel / tiles);
-      s.begin = static_cast<int>(rel - static_cast<int64_t>(s.head) * tiles);
-      s.end = static_cast<int>(min(static_cast<int64_t>(tiles), s.begin + (end - at)));
-      s.slot = s.begin == 0 && s.end == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (at == first ? 0 : 1);
-      at += s.end - s.begin;
-    } else {
-      s.entry = static_cast<int>(at / p.item_heads);
-      s.head = static_cast<int>(at - static_cast<int64_t>(s.entry) * p.item_heads);
-      s.slot = -1;
-      ++at;
+      s.batch = s.entry / p.row_tiles;
+      s.token0 = (s.entry - s.batch * p.row_tiles) * p.tile_tokens;
+      return true;
     }
-    s.batch = s.entry / p.row_tiles;
-    s.token0 = (s.entry - s.batch * p.row_tiles) * p.tile_tokens;
-    return true;
   }
 };
 
@@ -185,9 +194,9 @@ EB_DEVICE void publish_run(const Args& p, const int* cum, const Walk& walk) {
     Walk probe = walk;
     Segment s;
     int4 cut = make_int4(0, 0, 0, 0);
-    if (probe.next(p, cum, s)) cut = make_int4(s.entry, s.head, s.begin, cum[s.entry + 1] - cum[s.entry]);
+    if (probe.next(p, cum, s)) cut = make_int4(s.entry, s.head, s.begin, cum[s.entry + 1] - cum[s.entry] - p.item_cost);
     reinterpret_cast<int4*>(p.cuts)[blockIdx.x] = cut;
-    if (blockIdx.x == 0) *p.run = static_cast<int>(run_tiles(p, cum[p.batch * p.row_tiles], gridDim.x));
+    if (blockIdx.x == 0) *p.run = run_units(p, cum[p.batch * p.row_tiles], gridDim.x);
   }
   // Every CTA takes a share of each such entry: the last tiles of a ragged batch may all be empty.
   const int entries = p.batch * p.row_tiles;

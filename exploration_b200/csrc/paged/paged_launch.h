@@ -80,7 +80,6 @@ inline void set_rows(Args& args, int most, int key_tile) {
   args.row_tile = args.tile_tokens * part;
   args.row_tiles = cdiv(args.tokens, args.tile_tokens);
   args.key_tile = key_tile;
-  args.min_run = 1;
 }
 
 // The split of one call: CTAs, and the workspace of the cut items. The
@@ -90,12 +89,13 @@ struct Split {
   int ctas = 0;
   at::Tensor space;
 
-  // `whole_tiles`: items of at most so many key tiles are not cut.
-  Split(Args& args, int wanted, int whole_tiles) {
+  // `whole_tiles`: items of at most so many key tiles are not cut. `item_cost`: see Args.
+  Split(Args& args, int wanted, int whole_tiles, int item_cost) {
     const int64_t entries = static_cast<int64_t>(args.batch) * args.row_tiles;
     const int64_t items = entries * args.item_heads;
     const int64_t longest = cdiv64(static_cast<int64_t>(args.width) * args.page, args.key_tile);
-    args.flat = entries <= kMaxEntries && longest > whole_tiles;
+    args.item_cost = item_cost;
+    args.flat = entries <= kMaxEntries && longest > whole_tiles && items * (longest + item_cost) < (1LL << 31);
     if (!args.flat) {
       TORCH_CHECK(items < (1LL << 31), "paged_attention: too many rows");
       ctas = static_cast<int>(items);

@@ -38,6 +38,7 @@ using namespace paged;
 using namespace sm100;
 
 constexpr int kRows = 16;
+constexpr int kItemCost = 2;   // of an item's start and end, in tiles
 constexpr int kTile = 64;
 // Items of up to 1,024 keys are not cut, because joining costs a launch: 4 sequences of
 // up to 517 keys, 4 heads of 64, take one kernel of 8.1 us whole, 5.3 + 3.5 us cut.
@@ -341,7 +342,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 
 template <typename T, int D>
 void launch(Args& args, int sms, cudaStream_t stream) {
-  const Split split(args, sms * RowsConfig<D>::kCtas, kWholeTiles);
+  const Split split(args, sms * RowsConfig<D>::kCtas, kWholeTiles, kItemCost);
   const CUtensorMap tk = make_pool_map(args, args.k, std::is_same_v<T, __half>, kTile);
   const CUtensorMap tv = make_pool_map(args, args.v, std::is_same_v<T, __half>, kTile);
   const size_t smem = sizeof(RowsSmem<D>) + 1024;

@@ -27,6 +27,7 @@ namespace {
 using namespace paged;
 
 constexpr int kWarps = 4;
+constexpr int kItemCost = 2;   // of an item's start and end, in tiles
 constexpr int kTile = 64;
 constexpr int kWholeTiles = 16;   // items of up to 1,024 keys are not cut (as in the few-row kernel)
 constexpr int kWarpKeys = kTile / kWarps;
@@ -214,7 +215,7 @@ paged_simt_kernel(Args p) {
 
 template <typename T, int DP, int R>
 void launch(Args& args, int sms, cudaStream_t stream) {
-  const Split split(args, sms * 4, kWholeTiles);
+  const Split split(args, sms * 4, kWholeTiles, kItemCost);
   paged_simt_kernel<T, DP, R><<<split.ctas, kWarps * 32, 0, stream>>>(args);
   EB_CUDA_CHECK(cudaGetLastError());
   count_launch(1);

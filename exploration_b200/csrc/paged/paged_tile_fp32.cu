@@ -29,6 +29,7 @@ namespace {
 using namespace paged;
 
 constexpr int kRows = 64;
+constexpr int kItemCost = 1;   // of an item's start and end, in tiles
 constexpr int kTile = 64;
 constexpr int kThreads = 128;
 
@@ -209,7 +210,7 @@ paged_tile_fp32_kernel(Args p) {
 
 template <int D>
 void launch(Args& args, int sms, cudaStream_t stream) {
-  const Split split(args, sms * (D == 64 ? 3 : 2), 0);
+  const Split split(args, sms * (D == 64 ? 3 : 2), 0, kItemCost);
   const size_t smem = sizeof(TileSmem<D>);
   auto kernel = paged_tile_fp32_kernel<D>;
   allow_smem(reinterpret_cast<const void*>(kernel), smem);
