@@ -83,7 +83,7 @@ struct alignas(1024) ChunkSmem {
   int abort;
   int clear_stage;
   float ml[kM][2];
-  int cum[kMaxEntries + 1];
+  Prefix table;
 };
 
 // Positions in the two rings and of the barriers' phases, carried across items.
@@ -173,15 +173,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     fence_barrier_init();
   }
   if (warp == 2) tmem_alloc(&sm.tmem_base, kTmemCols);
-  if (p.flat) build_prefix(p, sm.cum);
+  if (p.flat) build_prefix(p, sm.table);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = sm.tmem_base;
   Walk walk;
-  walk.start(p, sm.cum);
-  publish_run<T>(p, sm.cum, walk);
+  walk.start(p, sm.table);
+  publish_run<T>(p, sm.table, walk);
   Segment s;
   const int half_tokens = kM / p.group;         // tokens of one warpgroup's rows
   const int half_rows = half_tokens * p.group;
@@ -200,10 +200,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     Ring ring;            // K and V advance together
     int q_loads = 0, tiles_issued = 0;
     bool ok = true;
-    while (ok && walk.next(p, sm.cum, s)) {
-      finish_segment(p, s, lane);
-      if (s.begin == s.end) continue;
+    while (ok && walk.next(p, sm.table, s)) {
+      // The first entries are on their way before the limit is known (the table has them all).
+      const int* table = p.tables + static_cast<int64_t>(s.batch) * p.width;
       const int kv_head = s.head / p.head_div;
+      auto entry = [&](int page) { return page < p.width ? table[page] : -1; };
+      int base = p.flat ? (s.begin * kTile) >> p.page_shift : 0;
+      int ids = entry(base + lane), ahead = entry(base + 32 + lane);
+      finish_segment(p, sm.table, s, lane);
+      if (s.begin == s.end) continue;
       if (q_loads > 0 && !__all_sync(0xffffffffu, wait_tight(&sm.q_empty, (q_loads - 1) & 1, abort, err, kSiteQFull)))
         break;
       const int halves = split_rows(s) ? 2 : 1;
@@ -216,11 +221,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
                         s.batch);
       }
       ++q_loads;
-      const int* table = p.tables + static_cast<int64_t>(s.batch) * p.width;
-      const int last_page = (s.limit - 1) >> p.page_shift;
-      auto entry = [&](int page) { return page <= last_page ? table[page] : -1; };
-      int base = (s.begin * kTile) >> p.page_shift;
-      int ids = entry(base + lane), ahead = entry(base + 32 + lane);
       for (int tile = s.begin; tile < s.end; ++tile) {
         const int key0 = tile * kTile;
         const int boxes = min(boxes_tile, cdiv(s.limit - key0, box));
@@ -275,8 +275,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     Ring kr, vr, sr, pr;    // key and value stages, score buffers to fill and weights to use
     int segments = 0, cleared = 0;
     bool ok = true;
-    while (ok && walk.next(p, sm.cum, s)) {
-      finish_segment(p, s, lane);
+    while (ok && walk.next(p, sm.table, s)) {
+      finish_segment(p, sm.table, s, lane);
       if (s.begin == s.end) continue;
       const bool dual = split_rows(s);
       const int tiles = s.end - s.begin, steps = dual ? 2 * tiles : tiles;
@@ -349,8 +349,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     // Rows past an item's limit in its last value tile: cleared when warp 1 has seen the tile arrive.
     int cleared = 0;
     bool ok = true;
-    while (ok && walk.next(p, sm.cum, s)) {
-      finish_segment(p, s, lane);
+    while (ok && walk.next(p, sm.table, s)) {
+      finish_segment(p, sm.table, s, lane);
       if (s.begin == s.end || s.limit >= s.end * kTile) continue;
       ok = __all_sync(0xffffffffu, mbar_wait(&sm.v_ragged, cleared & 1, abort, err, kSiteKvFull));
       if (!ok) break;
@@ -384,8 +384,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       tc_fence_after();
       return met;
     };
-    while (ok && walk.next(p, sm.cum, s)) {
-      finish_segment(p, s, lane);
+    while (ok && walk.next(p, sm.table, s)) {
+      finish_segment(p, sm.table, s, lane);
       const bool dual = split_rows(s);
       const int first = dual ? w * half_tokens : 0;
       const int token = s.token0 + first + row / p.group;

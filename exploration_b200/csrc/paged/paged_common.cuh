@@ -29,7 +29,12 @@ namespace eb {
 namespace paged {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxEntries = 2048;   // entries whose tile counts fit the CTA's shared prefix table
+constexpr int kMaxEntries = 1024;   // entries that fit a CTA's shared table
+
+struct Prefix {
+  int cum[kMaxEntries + 1];         // units of the entries before
+  int limit[kMaxEntries];           // keys
+};
 
 struct Args {
   const void* q;          // [batch, tokens, heads, dim], dense
@@ -88,17 +93,24 @@ EB_DEVICE int entry_limit_warp(const Args& p, int entry, int lane) {
 // Units of an item of `limit` keys: its tiles, then its fixed cost.
 EB_DEVICE int entry_units(const Args& p, int limit) { return limit > 0 ? cdiv(limit, p.key_tile) + p.item_cost : 0; }
 
-// Prefix of the entries' units into cum[0 .. entries] (shared memory); all threads.
-EB_DEVICE void build_prefix(const Args& p, int* cum) {
+// Limits of the entries and prefix of their units; all threads.
+EB_DEVICE void build_prefix(const Args& p, Prefix& table) {
   const int entries = p.batch * p.row_tiles;
+  int* cum = table.cum;
   if (p.tile_tokens <= 16) {
-    for (int e = threadIdx.x; e < entries; e += blockDim.x)
-      cum[e + 1] = entry_units(p, entry_limit(p, e));
+    for (int e = threadIdx.x; e < entries; e += blockDim.x) {
+      const int n = entry_limit(p, e);
+      table.limit[e] = n;
+      cum[e + 1] = entry_units(p, n);
+    }
   } else {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int e = warp; e < entries; e += blockDim.x >> 5) {
       const int n = entry_limit_warp(p, e, lane);
-      if (lane == 0) cum[e + 1] = entry_units(p, n);
+      if (lane == 0) {
+        table.limit[e] = n;
+        cum[e + 1] = entry_units(p, n);
+      }
     }
   }
   if (threadIdx.x == 0) cum[0] = 0;
@@ -127,13 +139,14 @@ EB_DEVICE int run_units(const Args& p, int total, int ctas) {
   return all / ctas + (all % ctas != 0);
 }
 
-// Walks the segments of one CTA's run. `cum` is unused when flat == 0.
+// Walks the segments of one CTA's run. `table` is unused when flat == 0.
 struct Walk {
   int at, end, first;
   int entry_hint;
 
-  EB_DEVICE void start(const Args& p, const int* cum) {
+  EB_DEVICE void start(const Args& p, const Prefix& table) {
     if (p.flat) {
+      const int* cum = table.cum;
       const int total = cum[p.batch * p.row_tiles];
       const int run = run_units(p, total, gridDim.x), all = total * p.item_heads;
       at = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * run, static_cast<int64_t>(all)));
@@ -149,7 +162,8 @@ struct Walk {
 
   // The next segment, or false. Uniform over the threads that call it. In the
   // one-item form the segment may be empty (begin == end, slot -1): the output is zero.
-  EB_DEVICE bool next(const Args& p, const int* cum, Segment& s) {
+  EB_DEVICE bool next(const Args& p, const Prefix& table, Segment& s) {
+    const int* cum = table.cum;
     while (true) {
       if (at >= end) return false;
       const int here = at;
@@ -188,13 +202,14 @@ struct Walk {
 
 // What the combine kernel needs, and the rows of entries without any key. All threads, after walk.start().
 template <typename T>
-EB_DEVICE void publish_run(const Args& p, const int* cum, const Walk& walk) {
+EB_DEVICE void publish_run(const Args& p, const Prefix& table, const Walk& walk) {
   if (!p.flat) return;
+  const int* cum = table.cum;
   if (threadIdx.x == 0) {
     Walk probe = walk;
     Segment s;
     int4 cut = make_int4(0, 0, 0, 0);
-    if (probe.next(p, cum, s)) cut = make_int4(s.entry, s.head, s.begin, cum[s.entry + 1] - cum[s.entry] - p.item_cost);
+    if (probe.next(p, table, s)) cut = make_int4(s.entry, s.head, s.begin, cum[s.entry + 1] - cum[s.entry] - p.item_cost);
     reinterpret_cast<int4*>(p.cuts)[blockIdx.x] = cut;
     if (blockIdx.x == 0) *p.run = run_units(p, cum[p.batch * p.row_tiles], gridDim.x);
   }
@@ -216,9 +231,11 @@ EB_DEVICE void publish_run(const Args& p, const int* cum, const Walk& walk) {
 }
 
 // Limit of a segment's item, and for the one-item form its tiles; every thread of a warp calls it.
-EB_DEVICE void finish_segment(const Args& p, Segment& s, int lane) {
-  s.limit = entry_limit_warp(p, s.entry, lane);
-  if (!p.flat) {
+EB_DEVICE void finish_segment(const Args& p, const Prefix& table, Segment& s, int lane) {
+  if (p.flat) {
+    s.limit = table.limit[s.entry];
+  } else {
+    s.limit = entry_limit_warp(p, s.entry, lane);
     s.begin = 0;
     s.end = cdiv(s.limit, p.key_tile);
   }

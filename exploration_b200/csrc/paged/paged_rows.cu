@@ -67,7 +67,7 @@ struct alignas(1024) RowsSmem {
   float ml[kConsumers][kRows][2];
   uint64_t full[kStages], empty[kStages];
   int abort;
-  int cum[kMaxEntries + 1];
+  Prefix table;
 };
 
 template <typename T, int D>
@@ -89,12 +89,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     sm.abort = 0;
     fence_barrier_init();
   }
-  if (p.flat) build_prefix(p, sm.cum);
+  if (p.flat) build_prefix(p, sm.table);
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Walk walk;
-  walk.start(p, sm.cum);
-  publish_run<T>(p, sm.cum, walk);
+  walk.start(p, sm.table);
+  publish_run<T>(p, sm.table, walk);
   Segment s;
 
   if (warp == kConsumers) {
@@ -107,14 +107,14 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     }
     int issued = 0;
     bool ok = true;
-    while (ok && walk.next(p, sm.cum, s)) {
-      finish_segment(p, s, lane);
+    while (ok && walk.next(p, sm.table, s)) {
+      // The first entries are on their way before the limit is known (the table has them all).
       const int* table = p.tables + static_cast<int64_t>(s.batch) * p.width;
       const int kv_head = s.head / p.head_div;
-      const int last_page = (s.limit - 1) >> p.page_shift;
-      auto entry = [&](int page) { return page <= last_page ? table[page] : -1; };
-      int base = (s.begin * kTile) >> p.page_shift;
+      auto entry = [&](int page) { return page < p.width ? table[page] : -1; };
+      int base = p.flat ? (s.begin * kTile) >> p.page_shift : 0;
       int ids = entry(base + lane), ahead = entry(base + 32 + lane);
+      finish_segment(p, sm.table, s, lane);
       for (int tile = s.begin; tile < s.end; ++tile) {
         const int stage = issued % kStages;
         if (issued >= kStages && !__all_sync(0xffffffffu, wait_tight(&sm.empty[stage], ((issued / kStages) - 1) & 1,
@@ -159,7 +159,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   const T* q = static_cast<const T*>(p.q);
   int done = 0;
   bool ok = true;
-  while (ok && walk.next(p, sm.cum, s)) {
+  while (ok && walk.next(p, sm.table, s)) {
     const int rows = min(p.tile_tokens, p.tokens - s.token0) * p.group;
     const int64_t row_base = static_cast<int64_t>(s.batch) * p.tokens + s.token0;
     const int r0 = lane >> 2, c0 = (lane & 3) * 2;

@@ -65,23 +65,23 @@ paged_simt_kernel(Args p) {
   constexpr int U = DP == 256 ? 4 : (DP == 32 ? 4 : 8);
   constexpr int kPass = NG * U;
   using Sum = std::conditional_t<sizeof(T) == 4, double, float>;
-  __shared__ int cum[kMaxEntries + 1];
+  __shared__ Prefix table;
   __shared__ float sm_ml[kWarps][R][2];
   __shared__ float sm_o[kWarps][R][DP];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int grp = lane / LK, d0 = (lane % LK) * VE;
   const int valid = p.dim - d0;                   // elements of this lane's vector that exist
   const bool vec = (p.dim & 3) == 0;
-  if (p.flat) build_prefix(p, cum);
+  if (p.flat) build_prefix(p, table);
   Walk walk;
-  walk.start(p, cum);
-  publish_run<T>(p, cum, walk);
+  walk.start(p, table);
+  publish_run<T>(p, table, walk);
   Segment s;
   const T* q = static_cast<const T*>(p.q);
   const T* kc = static_cast<const T*>(p.k);
   const T* vc = static_cast<const T*>(p.v);
-  while (walk.next(p, cum, s)) {
-    finish_segment(p, s, lane);
+  while (walk.next(p, table, s)) {
+    finish_segment(p, table, s, lane);
     const int rows = min(p.tile_tokens, p.tokens - s.token0) * p.group;
     const int64_t row_base = static_cast<int64_t>(s.batch) * p.tokens + s.token0;
     float qr[R][VE], o[R][VE], m[R], l[R];
@@ -100,12 +100,12 @@ paged_simt_kernel(Args p) {
       m[r] = kNegInf;
       l[r] = 0.f;
     }
-    const int* table = p.tables + static_cast<int64_t>(s.batch) * p.width;
+    const int* pages = p.tables + static_cast<int64_t>(s.batch) * p.width;
     const int64_t head_step = static_cast<int64_t>(p.page) * p.dim;
     const int kv_head = s.head / p.head_div;
     auto page_of = [&](int tile) {
       const int key = tile * kTile + warp * kWarpKeys;
-      return tile < s.end && key < s.limit ? table[key >> p.page_shift] : -1;
+      return tile < s.end && key < s.limit ? pages[key >> p.page_shift] : -1;
     };
     int next_id = page_of(s.begin);
     for (int tile = s.begin; tile < s.end; ++tile) {

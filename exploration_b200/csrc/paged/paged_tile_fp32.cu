@@ -40,7 +40,7 @@ struct TileSmem {
   float q[kRows * kLd];
   float k[kTile * kLd];                     // then the weights [row][key]
   float v[kTile * D];
-  int cum[kMaxEntries + 1];
+  Prefix table;
 };
 
 EB_DEVICE void copy16(float* dst, const float* src, bool real) {
@@ -61,13 +61,13 @@ paged_tile_fp32_kernel(Args p) {
   static_assert(kRows * TileSmem<D>::kLdW <= kTile * TileSmem<D>::kLd, "the weights fit over the keys");
   const int lane = threadIdx.x & 31, rg = threadIdx.x >> 4, cg = threadIdx.x & 15;
   float* weights = sm.k;
-  if (p.flat) build_prefix(p, sm.cum);
+  if (p.flat) build_prefix(p, sm.table);
   Walk walk;
-  walk.start(p, sm.cum);
-  publish_run<float>(p, sm.cum, walk);
+  walk.start(p, sm.table);
+  publish_run<float>(p, sm.table, walk);
   Segment s;
-  while (walk.next(p, sm.cum, s)) {
-    finish_segment(p, s, lane);
+  while (walk.next(p, sm.table, s)) {
+    finish_segment(p, sm.table, s, lane);
     const int rows = min(p.tile_tokens, p.tokens - s.token0) * p.group;
     const int64_t row_base = static_cast<int64_t>(s.batch) * p.tokens + s.token0;
     auto query_row = [&](int r) {   // element offset of a row of the queries or the result
