@@ -262,9 +262,9 @@ EB_DEVICE void choose(const SelectArgs& p, int group, int lane, const float (*to
 }
 
 // Candidate i of a beam with logit x: its total score.
-EB_DEVICE void offer(const SelectArgs& p, int row, float lse, int i, float x, int t, float& total, int& token) {
-  const float base = p.scores[row];
-  if (p.finished[row]) {
+EB_DEVICE void offer(const SelectArgs& p, float base, bool ended, float lse, int i, float x, int t, float& total,
+                     int& token) {
+  if (ended) {
     total = i == 0 ? base : kNegInf;
     token = p.eos;
   } else if (!isfinite(lse)) {
@@ -290,11 +290,13 @@ beam_select_small_kernel(SelectArgs p) {
     const T* logits = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.vocab;
     LaneLogits<T> x;
     x.load(logits, aligned_start(logits), p.vocab, lane);
+    const float score = p.scores[row];
+    const bool ended = p.finished[row];
     float m, s, peak;
     x.sum(m, s, peak);
     const float lse = m + logf(s);
     x.best(p.keep, p.vocab, lane, logits, peak, list[warp], [&](int i, float value, int t) {
-      if (lane == 0) offer(p, row, lse, i, value, t, total[warp][i], token[warp][i]);
+      if (lane == 0) offer(p, score, ended, lse, i, value, t, total[warp][i], token[warp][i]);
     });
   }
   __syncthreads();
@@ -361,6 +363,22 @@ beam_select_chunk_kernel(SelectArgs p) {
 // One warp: a beam's sums and best logits from its chunks'.
 EB_DEVICE void join_beam(const SelectArgs& p, int row, int lane, float* total, int* token) {
   const int64_t base = static_cast<int64_t>(row) * p.chunks;
+  // Everything that the beam needs is read at once.
+  const float score = p.scores[row];
+  const bool ended = p.finished[row];
+  const int entries = p.chunks * p.keep;
+  uint64_t keys[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int e = i * 32 + lane;
+    keys[i] = 0;
+    if (e < entries) {
+      const int t = p.part_t[base * p.keep + e];
+      const float v = p.part_x[base * p.keep + e];
+      if (t != INT_MAX)
+        keys[i] = static_cast<uint64_t>(ordered(v + 0.f)) << 32 | (0xffffffffu - static_cast<uint32_t>(t));
+    }
+  }
   float m = kNegInf;
   for (int c = lane; c < p.chunks; c += 32) m = fmaxf(m, p.part_ms[(base + c) * 2]);
   m = warp_max(m);
@@ -374,22 +392,9 @@ EB_DEVICE void join_beam(const SelectArgs& p, int row, int lane, float* total, i
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   const float lse = m + logf(static_cast<float>(sum));
-  const int entries = p.chunks * p.keep;
   if (entries <= 32 * kHeld) {
-    uint64_t keys[kHeld];
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      const int e = i * 32 + lane;
-      keys[i] = 0;
-      if (e < entries) {
-        const int t = p.part_t[base * p.keep + e];
-        if (t != INT_MAX)
-          keys[i] = static_cast<uint64_t>(ordered(p.part_x[base * p.keep + e])) << 32 |
-                    (0xffffffffu - static_cast<uint32_t>(t));
-      }
-    }
     pick_from(p.keep, keys, [&](int i, float value, int t) {
-      if (lane == 0) offer(p, row, lse, i, value, t, total[i], token[i]);
+      if (lane == 0) offer(p, score, ended, lse, i, value, t, total[i], token[i]);
     });
     return;
   }
@@ -421,7 +426,7 @@ EB_DEVICE void join_beam(const SelectArgs& p, int row, int lane, float* total, i
     const uint32_t top = __reduce_max_sync(0xffffffffu, mine == INT_MAX ? 0u : key);
     const int cand = mine != INT_MAX && key == top ? mine : INT_MAX;
     const int first = __reduce_min_sync(0xffffffffu, cand);
-    if (lane == 0) offer(p, row, lse, round, unordered(top), first, total[round], token[round]);
+    if (lane == 0) offer(p, score, ended, lse, round, unordered(top), first, total[round], token[round]);
     if (cand == first && first != INT_MAX) {
       last_key = key;
       last_t = mine;

@@ -58,6 +58,7 @@ struct Args {
   int key_tile;           // keys of a tile
   int flat;               // 1: equal runs of the tile list; 0: one item a CTA (too many entries for the table)
   int item_cost;          // what starting and finishing an item costs, in tiles of work
+  int vectors;            // rows and pools allow loads of four elements (general kernel)
   float scale_log2;       // log2(e) / sqrt(dim)
 };
 

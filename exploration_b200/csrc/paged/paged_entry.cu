@@ -78,6 +78,9 @@ at::Tensor paged_attention(const at::Tensor& q_in, const at::Tensor& k_cache, co
   args.page = k_cache.size(2);
   args.page_shift = __builtin_ctz(args.page);
   args.width = tables.size(1);
+  const uintptr_t four = 4 * q.element_size();
+  args.vectors = args.dim % 4 == 0 && reinterpret_cast<uintptr_t>(args.q) % four == 0 &&
+                 reinterpret_cast<uintptr_t>(args.k) % four == 0 && reinterpret_cast<uintptr_t>(args.v) % four == 0;
   args.scale_log2 = static_cast<float>(paged::kLog2e / std::sqrt(static_cast<double>(args.dim)));
   auto stream = at::cuda::getCurrentCUDAStream();
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;

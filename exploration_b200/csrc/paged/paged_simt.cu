@@ -71,7 +71,7 @@ paged_simt_kernel(Args p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int grp = lane / LK, d0 = (lane % LK) * VE;
   const int valid = p.dim - d0;                   // elements of this lane's vector that exist
-  const bool vec = (p.dim & 3) == 0;
+  const bool vec = p.vectors != 0;
   if (p.flat) build_prefix(p, table);
   Walk walk;
   walk.start(p, table);

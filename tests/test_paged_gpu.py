@@ -135,6 +135,26 @@ def test_attention_extreme_logits(new, dtype):
     check_attention(q2, k2, v, tables, positions)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 5, 40])
+def test_attention_off_the_vector_grid(new, dtype):
+    """Queries and pools that start between 16-byte boundaries, and strided queries."""
+    lengths = [90, 300]
+    k, v, tables = make_cache(lengths, 2, 64, 16, dtype)
+    q, positions = queries(2, new, 4, 64, dtype), tail_positions(lengths, [new, new], new)
+
+    def shifted(t):
+        base = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+        base[1:] = t.flatten()
+        return base[1:].view(t.shape)
+
+    check_attention(shifted(q), k, v, tables, positions)
+    check_attention(q, shifted(k), shifted(v), tables, positions)
+    wide = torch.cat((q, q), 2)[:, :, 4:]
+    assert not wide.is_contiguous()
+    check_attention(wide, k, v, tables, positions)
+
+
 def test_attention_split_is_deterministic_and_streams():
     lengths = [5000, 20, 3000]
     k, v, tables = make_cache(lengths, 4, 64, 64, torch.bfloat16)
