@@ -28,7 +28,7 @@
 //
 // Measured: 2,048 tokens over 65,536 keys, 16 heads of 64, bf16: 0.64 ms in a short
 // burst (850 TFLOP/s), 0.76 ms sustained under the power cap (713); ragged chunks of
-// 1,111 tokens over up to 8,191 keys, 32/8 heads of 128, fp16: 0.42 and 0.47 ms (721).
+// 1,111 tokens over up to 8,191 keys, 32/8 heads of 128, fp16: 0.355 and 0.41 ms (824).
 // At head dim 64 a step is bound by the softmax instructions of two warps an SM
 // sub-partition (their special-function share alone is 2,048 cycles of 2,500) and the
 // hand-overs around them; at 128 by the chain weights -> P V -> next S -> softmax

@@ -18,15 +18,16 @@ enum class Path { kCudaCore, kTileFp32, kRows, kChunk };
 // The kernel of a call. Head dims 64 and 128 (one or two 128-byte swizzle spans of
 // a 16-bit type) have kernels of their own: up to 16 rows of a key head are bound
 // by the read of the cache, more by arithmetic. fp32 takes the general kernel for
-// few rows (0.16 ms for 2 x 60,001 keys, 94% of the measured copy bandwidth) and
-// the tiled one for many.
+// up to four rows and the tiled one for more (four sequences over 30,000 keys, 16
+// heads of 64: 4 tokens 302 us in the general kernel; 12 tokens 941 us there, 364 us
+// in tiles).
 Path choose(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache) {
   const int64_t dim = q.size(3);
   auto aligned = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; };
   if ((dim != 64 && dim != 128) || !aligned(q) || !aligned(k_cache) || !aligned(v_cache)) return Path::kCudaCore;
-  const bool few = q.size(1) * (q.size(2) / k_cache.size(1)) <= 16;
-  if (q.scalar_type() == at::kFloat) return few ? Path::kCudaCore : Path::kTileFp32;
-  return few ? Path::kRows : Path::kChunk;
+  const int64_t rows = q.size(1) * (q.size(2) / k_cache.size(1));
+  if (q.scalar_type() == at::kFloat) return rows <= 4 ? Path::kCudaCore : Path::kTileFp32;
+  return rows <= 16 ? Path::kRows : Path::kChunk;
 }
 
 template <typename T>

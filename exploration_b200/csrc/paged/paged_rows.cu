@@ -13,10 +13,10 @@
 // tcgen05 would cost here; arithmetic hides under the loads.
 //
 // Measured: one token of 64 sequences of 17 to 16,384 keys, 32/8 heads of 128,
-// bf16 (2.15 GB): 0.352 ms, 6.1 TB/s, 93% of the measured copy bandwidth. Five
-// tokens of 16 sequences of up to 4,099 keys, 16 heads of 64, fp16 (148 MB): 31.4 us
-// of kernel, bound by its start (positions, tables, first tiles: 4.5 us) and by the
-// joining launch after it (5 us).
+// bf16 (2.15 GB): 0.330 to 0.344 ms, 6.3 to 6.5 TB/s, 95 to 99% of the measured copy
+// bandwidth. Five tokens of 16 sequences of up to 4,099 keys, 16 heads of 64, fp16
+// (148 MB): 30 us of kernel, bound by its start (positions, tables, first tiles:
+// 4 us) and by the joining launch after it (5 us).
 //
 // Keys past an item's limit are masked, their values cleared in the fragments:
 // a page's unwritten rows may hold anything.

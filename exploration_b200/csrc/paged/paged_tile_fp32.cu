@@ -1,10 +1,11 @@
-// Attention of a chunk of new tokens over a paged cache in fp32 (head dim 64 or
-// 128, more than 16 rows of a key head): IEEE fp32 products, no TF32.
+// Attention of new tokens over a paged cache in fp32 (head dim 64 or 128, more than
+// four rows of a key head): IEEE fp32 products, no TF32.
 //
 // Bound by the fp32 pipe (75 TFLOP/s): every product comes from registers that
 // 12 16-byte shared-memory loads fill for 128 multiply-adds. One CTA of 128
-// threads takes 64 rows and walks 64-key tiles; a thread owns 8 rows x 4 keys of
-// the scores and 8 rows x D / 16 columns of the result, the 16 threads of a row
+// threads takes 8 RPT rows (RPT 8, or 4 or 2 when there are no more) and walks
+// 64-key tiles; a thread owns RPT rows x 4 keys of the scores and RPT rows x D / 16
+// columns of the result, the 16 threads of a row
 // sit in half a warp (row maxima and sums by shuffles). Weights go through
 // shared memory, over the keys that they came from. Two or three CTAs an SM hide
 // each other's loads. The products of a score are added from the last element to
@@ -28,13 +29,13 @@ namespace {
 
 using namespace paged;
 
-constexpr int kRows = 64;
 constexpr int kItemCost = 1;   // of an item's start and end, in tiles
 constexpr int kTile = 64;
 constexpr int kThreads = 128;
 
-template <int D>
+template <int D, int RPT>
 struct TileSmem {
+  static constexpr int kRows = 8 * RPT;
   static constexpr int kLd = D + 4;         // row pitch: eight rows reach all banks
   static constexpr int kLdW = kTile + 4;
   float q[kRows * kLd];
@@ -52,13 +53,18 @@ EB_DEVICE void copies_done() {
   asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
 }
 
-template <int D>
-__global__ void __launch_bounds__(kThreads, D == 64 ? 3 : 2)
+// CTAs an SM, within registers (64 rows) and shared memory.
+template <int D, int RPT>
+constexpr int kCtas = D == 64 ? (RPT == 8 ? 3 : 4) : 2;
+
+template <int D, int RPT>
+__global__ void __launch_bounds__(kThreads, (kCtas<D, RPT>))
 paged_tile_fp32_kernel(Args p) {
   extern __shared__ __align__(16) uint8_t raw[];
-  TileSmem<D>& sm = *reinterpret_cast<TileSmem<D>*>(raw);
-  constexpr int kLd = TileSmem<D>::kLd, kLdW = TileSmem<D>::kLdW, kQuads = D / 4, kCols = D / 64;
-  static_assert(kRows * TileSmem<D>::kLdW <= kTile * TileSmem<D>::kLd, "the weights fit over the keys");
+  using Smem = TileSmem<D, RPT>;
+  Smem& sm = *reinterpret_cast<Smem*>(raw);
+  constexpr int kRows = Smem::kRows, kLd = Smem::kLd, kLdW = Smem::kLdW, kQuads = D / 4, kCols = D / 64;
+  static_assert(kRows * kLdW <= kTile * kLd, "the weights fit over the keys");
   const int lane = threadIdx.x & 31, rg = threadIdx.x >> 4, cg = threadIdx.x & 15;
   float* weights = sm.k;
   if (p.flat) build_prefix(p, sm.table);
@@ -78,16 +84,16 @@ paged_tile_fp32_kernel(Args p) {
       const int r = i / kQuads, d = (i % kQuads) * 4;
       copy16(&sm.q[r * kLd + d], static_cast<const float*>(p.q) + query_row(r < rows ? r : 0) + d, r < rows);
     }
-    int pos[8], low = INT_MAX;
+    int pos[RPT], low = INT_MAX;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = rg * 8 + i;
+    for (int i = 0; i < RPT; ++i) {
+      const int r = rg * RPT + i;
       pos[i] = r < rows ? p.positions[row_base + r / p.group] : -1;
       if (pos[i] >= 0) low = min(low, pos[i]);
     }
-    float o[8][4 * kCols], m[8], l[8];
+    float o[RPT][4 * kCols], m[RPT], l[RPT];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < RPT; ++i) {
       m[i] = kNegInf;
       l[i] = 0.f;
 #pragma unroll
@@ -109,10 +115,10 @@ paged_tile_fp32_kernel(Args p) {
       }
       copies_done();
       __syncthreads();
-      // Scores: rows rg * 8 + i, keys cg + 16 j.
-      float a[8][4];
+      // Scores: rows rg * RPT + i, keys cg + 16 j.
+      float a[RPT][4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < RPT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) a[i][j] = 0.f;
 #pragma unroll 2
@@ -121,8 +127,8 @@ paged_tile_fp32_kernel(Args p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) kx[j] = *reinterpret_cast<const float4*>(&sm.k[(cg + 16 * j) * kLd + d]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 qx = *reinterpret_cast<const float4*>(&sm.q[(rg * 8 + i) * kLd + d]);
+        for (int i = 0; i < RPT; ++i) {
+          const float4 qx = *reinterpret_cast<const float4*>(&sm.q[(rg * RPT + i) * kLd + d]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             a[i][j] = fmaf(qx.w, kx[j].w, a[i][j]);
@@ -134,7 +140,7 @@ paged_tile_fp32_kernel(Args p) {
       }
       const bool masked = key0 + kTile - 1 > low || key0 + kTile > s.limit;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < RPT; ++i) {
         float top = kNegInf;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -158,9 +164,9 @@ paged_tile_fp32_kernel(Args p) {
       }
       __syncthreads();   // the keys have been read
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < RPT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) weights[(rg * 8 + i) * kLdW + cg + 16 * j] = a[i][j];
+        for (int j = 0; j < 4; ++j) weights[(rg * RPT + i) * kLdW + cg + 16 * j] = a[i][j];
       __syncwarp();      // a warp's rows are its own: no other warp reads them
 #pragma unroll 2
       for (int key = 0; key < kTile; key += 4) {
@@ -171,8 +177,8 @@ paged_tile_fp32_kernel(Args p) {
           for (int c = 0; c < kCols; ++c)
             vx[t][c] = *reinterpret_cast<const float4*>(&sm.v[(key + t) * D + c * 64 + cg * 4]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 w = *reinterpret_cast<const float4*>(&weights[(rg * 8 + i) * kLdW + key]);
+        for (int i = 0; i < RPT; ++i) {
+          const float4 w = *reinterpret_cast<const float4*>(&weights[(rg * RPT + i) * kLdW + key]);
           const float wt[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int t = 0; t < 4; ++t)
@@ -187,8 +193,8 @@ paged_tile_fp32_kernel(Args p) {
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = rg * 8 + i;
+    for (int i = 0; i < RPT; ++i) {
+      const int r = rg * RPT + i;
 #pragma unroll
       for (int off = 8; off > 0; off >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
       if (r >= rows) continue;
@@ -208,11 +214,12 @@ paged_tile_fp32_kernel(Args p) {
   }
 }
 
-template <int D>
+template <int D, int RPT>
 void launch(Args& args, int sms, cudaStream_t stream) {
-  const Split split(args, sms * (D == 64 ? 3 : 2), 0, kItemCost);
-  const size_t smem = sizeof(TileSmem<D>);
-  auto kernel = paged_tile_fp32_kernel<D>;
+  set_rows(args, 8 * RPT, kTile);
+  const Split split(args, sms * kCtas<D, RPT>, 0, kItemCost);
+  const size_t smem = sizeof(TileSmem<D, RPT>);
+  auto kernel = paged_tile_fp32_kernel<D, RPT>;
   allow_smem(reinterpret_cast<const void*>(kernel), smem);
   kernel<<<split.ctas, kThreads, smem, stream>>>(args);
   EB_CUDA_CHECK(cudaGetLastError());
@@ -223,9 +230,17 @@ void launch(Args& args, int sms, cudaStream_t stream) {
 }  // namespace
 
 void paged_tile_fp32_launch(Args& args, int sms, cudaStream_t stream) {
-  set_rows(args, kRows, kTile);
-  if (args.dim == 64) return launch<64>(args, sms, stream);
-  return launch<128>(args, sms, stream);
+  // The smallest tile that takes all rows of a key head, or 64 rows: 16 tokens of four sequences
+  // over 30,000 keys, 16 heads of 64, take 364 us in tiles of 16 rows and 806 us in tiles of 64.
+  const int64_t rows = static_cast<int64_t>(args.heads / args.kv_heads) * args.tokens;
+  if (args.dim == 64) {
+    if (rows <= 16) return launch<64, 2>(args, sms, stream);
+    if (rows <= 32) return launch<64, 4>(args, sms, stream);
+    return launch<64, 8>(args, sms, stream);
+  }
+  if (rows <= 16) return launch<128, 2>(args, sms, stream);
+  if (rows <= 32) return launch<128, 4>(args, sms, stream);
+  return launch<128, 8>(args, sms, stream);
 }
 
 }  // namespace eb
