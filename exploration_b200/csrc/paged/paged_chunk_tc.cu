@@ -51,6 +51,7 @@
 #include "paged_common.cuh"
 #include "paged_launch.h"
 #include "paged_mma.cuh"
+#include "paged_phases.h"
 
 namespace eb {
 namespace {
@@ -78,7 +79,8 @@ struct alignas(1024) ChunkSmem {
   uint16_t v[kStages][kTile * D];
   uint64_t q_full, q_empty;
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[kBufs], p_full[kBufs], p_half[kBufs], o_done[2], join, v_ragged, v_clear;
+  uint64_t s_full[kBufs], p_full[kBufs], p_half[kBufs], join, v_ragged, v_clear;
+  uint64_t o_done[2][kProductBarriers];   // of each warpgroup, its products in turn (paged_phases.h)
   uint32_t tmem_base;
   int abort;
   int clear_stage;
@@ -148,6 +150,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   constexpr int kStages = ChunkSmem<D>::kStages, kBufs = ChunkSmem<D>::kBufs;
   constexpr bool kHalves = ChunkSmem<D>::kHalves;
   constexpr int kO = kTmemCols - 2 * D;          // first TMEM column of the accumulators
+  static_assert(kProductBarriers == 2, "the issuer keeps each warpgroup's turn in one bit");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort = &sm.abort;
   if (threadIdx.x == 0) {
@@ -164,8 +167,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       mbar_init(&sm.p_full[b], 128);
       mbar_init(&sm.p_half[b], 128);
     }
-    mbar_init(&sm.o_done[0], 1);
-    mbar_init(&sm.o_done[1], 1);
+    for (int w = 0; w < 2; ++w)
+      for (uint32_t b = 0; b < kProductBarriers; ++b) mbar_init(&sm.o_done[w][b], 1);
     mbar_init(&sm.join, 256);
     mbar_init(&sm.v_ragged, 1);
     mbar_init(&sm.v_clear, 1);
@@ -274,6 +277,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     const uint32_t id_pv = idesc_16(kBf16, kM, D, false, true);
     Ring kr, vr, sr, pr;    // key and value stages, score buffers to fill and weights to use
     int segments = 0, cleared = 0;
+    uint32_t turn = 0;      // bit w: barrier of warpgroup w's next product (product_phase)
     bool ok = true;
     while (ok && walk.next(p, sm.table, s)) {
       finish_segment(p, sm.table, s, lane);
@@ -334,7 +338,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             mma_ts_lo<kDescHi>(o_addr, p_addr + kk * 8, v_lo + kk * (2048 >> 4), id_pv, kk > 0 ? 1u : more);
           }
           if (!ok) break;
-          tc_commit(&sm.o_done[w]);
+          tc_commit(&sm.o_done[w][turn >> w & 1]);
+          turn ^= 1u << w;
           pr.next(kBufs);
           if (!dual || w == 1) {
             tc_commit(&sm.v_empty[vr.stage]);
@@ -375,6 +380,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     uint32_t done = 0;       // products this warpgroup has asked for
     uint32_t step0 = 0;      // steps of earlier items, both warpgroups'
     bool ok = true;
+    // The last product that this warpgroup asked for.
+    auto product_done = [&]() -> bool {
+      const Phase phase = product_phase(done - 1);
+      return __all_sync(0xffffffffu, wait_tight(&sm.o_done[w][phase.barrier], phase.parity, abort, err, kSiteODone));
+    };
     // Both warpgroups, bounded: TMEM accesses before it are ordered before those after it.
     auto join = [&]() -> bool {
       tc_fence_before();
@@ -438,7 +448,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           m = peak;
         }
         if (begun > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-          if (!__all_sync(0xffffffffu, wait_tight(&sm.o_done[w], (done - 1) & 1, abort, err, kSiteODone))) {
+          if (!product_done()) {
             ok = false;
             break;
           }
@@ -485,7 +495,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       if (!ok) break;
       step0 += (dual ? 2 : 1) * (s.end - s.begin);
       if (begun > 0) {
-        if (!__all_sync(0xffffffffu, wait_tight(&sm.o_done[w], (done - 1) & 1, abort, err, kSiteODone))) break;
+        if (!product_done()) break;
         tc_fence_after();
       }
       if (pos < 0) {   // a padding row: zero, no weight

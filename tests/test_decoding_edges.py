@@ -1,0 +1,76 @@
+"""Decoding operators and generation at their edges: what can be checked without a GPU."""
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+
+import exploration_b200
+
+PAGED = Path(exploration_b200.__file__).parent / "csrc" / "paged"
+
+# Runs the products of two softmax warpgroups in the issuer's order. At every wait of a warpgroup
+# (it has seen the scores of its newest step and asked for that step's product or not yet) each
+# number of finished products that is possible then is tried.
+PHASES = r"""
+#include <cstdio>
+#include <vector>
+#include "paged_phases.h"
+using namespace eb::paged;
+
+// mbarrier.try_wait.parity on a barrier with `phases` completed phases.
+static bool passes(uint32_t phases, uint32_t parity) { return (phases & 1) != parity; }
+
+// Completed phases of barrier b once `n` products of a warpgroup are complete.
+static uint32_t phases_of(uint32_t b, uint32_t n, uint32_t barriers) { return n / barriers + (b < n % barriers); }
+
+static long long wrong[2];
+static void look(uint32_t wanted, uint32_t done) {
+  const Phase p = product_phase(wanted);
+  wrong[0] += passes(phases_of(p.barrier, done, kProductBarriers), p.parity) != (done > wanted);
+  wrong[1] += passes(done, wanted & 1) != (done > wanted);      // one barrier a warpgroup
+}
+
+int main() {
+  for (int bufs = 2; bufs <= 3; ++bufs) {
+    uint32_t before[2] = {0, 0};           // products of earlier items (all complete)
+    for (int round = 0; round < 64; ++round) {
+      const int tiles = 1 + round % 7;
+      const bool dual = (round / 7) % 2;
+      const int steps = dual ? 2 * tiles : tiles;
+      for (int i = 0; i < steps; ++i) {
+        const int w = i & 1;
+        // The scores of step i are issued after product i - bufs: products up to it are complete.
+        uint32_t asked = 0, sure = 0;
+        for (int j = w; j < i; j += 2) { ++asked; sure += j <= i - bufs; }
+        if (asked > 0)                     // rescaling: waits for the product before this step's
+          for (uint32_t n = sure; n <= asked; ++n) look(before[w] + asked - 1, before[w] + n);
+        if (i + 2 >= steps)                // the item's end: waits for this step's product
+          for (uint32_t n = sure; n <= asked + 1; ++n) look(before[w] + asked, before[w] + n);
+      }
+      for (int i = 0; i < steps; ++i) ++before[i & 1];
+    }
+  }
+  std::printf("%lld %lld\n", wrong[0], wrong[1]);
+}
+"""
+
+
+def run_host_program(tmp_path, text):
+    """Compiles ``text`` against the kernels' host-checkable headers, runs it, returns its output's numbers."""
+    compiler = shutil.which("g++")
+    if compiler is None:
+        pytest.skip("no host compiler")
+    source, program = tmp_path / "check.cpp", tmp_path / "check"
+    source.write_text(text)
+    subprocess.run([compiler, "-std=c++17", "-O1", "-Wall", "-I", str(PAGED), str(source), "-o", str(program)],
+                   check=True, timeout=120)
+    done = subprocess.run([str(program)], check=True, capture_output=True, text=True, timeout=120)
+    return [int(x) for x in done.stdout.split()]
+
+
+def test_waits_for_products_are_never_ambiguous(tmp_path):
+    """A wait for a warpgroup's product passes exactly when that product is complete."""
+    wrong, wrong_with_one_barrier = run_host_program(tmp_path, PHASES)
+    assert wrong == 0
+    assert wrong_with_one_barrier > 0     # what the second barrier is for
