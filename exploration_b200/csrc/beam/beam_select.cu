@@ -1,7 +1,10 @@
 // Beam search's selection: the best `beams` continuations of a group of beams.
 //
 // Beam w at cumulative score c_w offers token t at c_w + (x_wt - lse_w) with
-// lse_w = log sum_t exp(x_wt); an ended beam offers only (eos, c_w). Inside a
+// lse_w = log sum_t exp(x_wt); an ended beam offers only (eos, c_w). With the
+// beam's largest logit m the difference is taken as (x_wt - m) - log sum_t
+// exp(x_wt - m), so that neither large logits nor a mask of the type's lowest
+// value (whose product with log2(e) is infinite) cost it any bits. Inside a
 // beam candidates are ordered by logit, then by token; across beams by score,
 // then by beam: rounding of the sum never reorders a beam's tokens, so each
 // beam's best `beams` logits are all that the final choice needs. A beam whose
@@ -12,7 +15,7 @@
 // (redux.sync on order-preserving integers). Up to 1,024 tokens one CTA a group
 // with a warp a beam does all in one launch. Longer rows are cut into chunks of
 // 8,192, one CTA each, whose sums and best K a second, overlapped launch joins:
-// sums of chunks in fp64, so lse does not depend on the cut beyond its rounding.
+// sums of chunks in fp64, so they do not depend on the cut beyond a rounding.
 // Measured: 8 x 8 beams of 100,003 bf16 logits (12.8 MB): 15.5 us for the chunks
 // (700 instructions a warp; 39 us when every round searched all logits), 26 us in all;
 // 4 x 4 beams of 256 tokens: 4.3 us of kernel.
@@ -117,16 +120,16 @@ struct LaneLogits {
     }
   }
 
-  // Maximum and sum of 2^((x - max) log2 e) over the warp; `peak`: of this lane alone.
+  // Maximum and sum of exp(x - max) over the warp; `peak`: of this lane alone.
   EB_DEVICE void sum(float& m, float& s, float& peak) const {
     peak = kNegInf;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) peak = fmaxf(peak, x[i]);
     m = warp_max(peak);
-    const float shift = finite_or_zero(m) * kLog2e;
+    const float ref = finite_or_zero(m);
     float part[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) part[i & 1] += ex2(fmaf(x[i], kLog2e, -shift));
+    for (int i = 0; i < kPerLane; ++i) part[i & 1] += ex2((x[i] - ref) * kLog2e);
     s = warp_sum(part[0] + part[1]);
   }
 
@@ -261,17 +264,17 @@ EB_DEVICE void choose(const SelectArgs& p, int group, int lane, const float (*to
   }
 }
 
-// Candidate i of a beam with logit x: its total score.
-EB_DEVICE void offer(const SelectArgs& p, float base, bool ended, float lse, int i, float x, int t, float& total,
-                     int& token) {
+// Candidate i of a beam with logit x, largest logit m and log_sum = log sum exp(x - m): its total score.
+EB_DEVICE void offer(const SelectArgs& p, float base, bool ended, float m, float log_sum, int i, float x, int t,
+                     float& total, int& token) {
   if (ended) {
     total = i == 0 ? base : kNegInf;
     token = p.eos;
-  } else if (!isfinite(lse)) {
+  } else if (!isfinite(m) || !isfinite(log_sum)) {
     total = kNegInf;
     token = i;
   } else {
-    const float sum = __fadd_rn(base, __fsub_rn(x, lse));
+    const float sum = __fadd_rn(base, __fsub_rn(__fsub_rn(x, m), log_sum));
     total = sum == sum ? sum : kNegInf;
     token = t;
   }
@@ -294,9 +297,9 @@ beam_select_small_kernel(SelectArgs p) {
     const bool ended = p.finished[row];
     float m, s, peak;
     x.sum(m, s, peak);
-    const float lse = m + logf(s);
+    const float log_sum = logf(s);
     x.best(p.keep, p.vocab, lane, logits, peak, list[warp], [&](int i, float value, int t) {
-      if (lane == 0) offer(p, score, ended, lse, i, value, t, total[warp][i], token[warp][i]);
+      if (lane == 0) offer(p, score, ended, m, log_sum, i, value, t, total[warp][i], token[warp][i]);
     });
   }
   __syncthreads();
@@ -383,7 +386,7 @@ EB_DEVICE void join_beam(const SelectArgs& p, int row, int lane, float* total, i
   for (int c = lane; c < p.chunks; c += 32) m = fmaxf(m, p.part_ms[(base + c) * 2]);
   m = warp_max(m);
   const float ref = finite_or_zero(m);
-  // The chunks' sums are added in fp64: lse depends on the cut by no more than its own rounding.
+  // The chunks' sums are added in fp64: the result depends on the cut by no more than its own rounding.
   double sum = 0.0;
   for (int c = lane; c < p.chunks; c += 32) {
     const float2 ms = *reinterpret_cast<const float2*>(p.part_ms + (base + c) * 2);
@@ -391,10 +394,10 @@ EB_DEVICE void join_beam(const SelectArgs& p, int row, int lane, float* total, i
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float lse = m + logf(static_cast<float>(sum));
+  const float log_sum = logf(static_cast<float>(sum));
   if (entries <= 32 * kHeld) {
     pick_from(p.keep, keys, [&](int i, float value, int t) {
-      if (lane == 0) offer(p, score, ended, lse, i, value, t, total[i], token[i]);
+      if (lane == 0) offer(p, score, ended, m, log_sum, i, value, t, total[i], token[i]);
     });
     return;
   }
@@ -426,7 +429,7 @@ EB_DEVICE void join_beam(const SelectArgs& p, int row, int lane, float* total, i
     const uint32_t top = __reduce_max_sync(0xffffffffu, mine == INT_MAX ? 0u : key);
     const int cand = mine != INT_MAX && key == top ? mine : INT_MAX;
     const int first = __reduce_min_sync(0xffffffffu, cand);
-    if (lane == 0) offer(p, score, ended, lse, round, unordered(top), first, total[round], token[round]);
+    if (lane == 0) offer(p, score, ended, m, log_sum, round, unordered(top), first, total[round], token[round]);
     if (cand == first && first != INT_MAX) {
       last_key = key;
       last_t = mine;

@@ -94,13 +94,16 @@ def select_reference(logits, scores, finished, eos):
     groups, beams, vocab = logits.shape
     keep = min(beams, vocab)
     x = logits.to(work_dtype(logits))
-    lse = x.logsumexp(-1, keepdim=True)
+    # x - logsumexp(x) from the distance to the largest logit: nothing is lost to the logits' size.
+    peak = x.amax(-1, keepdim=True)
+    log_sum = (x - peak).exp().sum(-1, keepdim=True).log()
+    alive = torch.isfinite(peak) & torch.isfinite(log_sum)
     best, token = x.sort(dim=-1, descending=True, stable=True)
     best, token = best[..., :keep], token[..., :keep]
-    total = scores[..., None] + (best - lse).float()
+    total = scores[..., None] + ((best - peak) - log_sum).float()
     rank = torch.arange(keep, device=logits.device)
-    total = torch.where(torch.isfinite(lse) & ~total.isnan(), total, NEG_INF)
-    token = torch.where(torch.isfinite(lse), token, rank)
+    total = torch.where(alive & ~total.isnan(), total, NEG_INF)
+    token = torch.where(alive, token, rank)
     first = rank == 0
     ended = finished[..., None]
     total = torch.where(ended, torch.where(first, scores[..., None], NEG_INF), total)

@@ -4,10 +4,12 @@ import subprocess
 from pathlib import Path
 
 import pytest
+import torch
 
-import exploration_b200
+import exploration_b200 as eb
+from exploration_b200.ops.beam import select_reference
 
-PAGED = Path(exploration_b200.__file__).parent / "csrc" / "paged"
+PAGED = Path(eb.__file__).parent / "csrc" / "paged"
 
 # Runs the products of two softmax warpgroups in the issuer's order. At every wait of a warpgroup
 # (it has seen the scores of its newest step and asked for that step's product or not yet) each
@@ -74,3 +76,23 @@ def test_waits_for_products_are_never_ambiguous(tmp_path):
     wrong, wrong_with_one_barrier = run_host_program(tmp_path, PHASES)
     assert wrong == 0
     assert wrong_with_one_barrier > 0     # what the second barrier is for
+
+
+def lowest_masked(dtype, vocab, spans):
+    """Logits whose ``spans`` hold the type's lowest value, and one beam that holds nothing else."""
+    logits = (3 * torch.randn(2, 3, vocab, generator=torch.Generator().manual_seed(vocab))).to(dtype)
+    for lo, hi in spans:
+        logits[:, :, lo:hi] = torch.finfo(dtype).min
+    logits[1, 1] = torch.finfo(dtype).min
+    return logits
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_select_with_the_types_lowest_value_as_a_mask(dtype):
+    scores, ended = -torch.rand(2, 3).cumsum(1), torch.zeros(2, 3, dtype=torch.bool)
+    for logits in (lowest_masked(dtype, 50, [(5, 20)]), lowest_masked(dtype, 50, [(2, 50)]),
+                   (torch.randn(2, 3, 50) + 2.0 ** 20).to(dtype)):
+        got = eb.beam_select(logits, scores, ended, -1)
+        want = select_reference(logits.double(), scores, ended, -1)
+        torch.testing.assert_close(got[0], want[0], atol=2e-5, rtol=0)
+        assert all(torch.equal(a, b) for a, b in zip(got[1:], want[1:]))

@@ -3,7 +3,8 @@ import pytest
 import torch
 
 import exploration_b200 as eb
-from tests.test_paged_gpu import check_attention, make_cache, queries, tail_positions
+from tests.test_decoding_edges import lowest_masked
+from tests.test_paged_gpu import check_attention, check_select, make_cache, queries, tail_positions
 
 pytestmark = pytest.mark.gpu
 SIXTEEN = [torch.float16, torch.bfloat16]
@@ -27,3 +28,22 @@ def test_attention_items_of_few_tiles(new, heads, kv, dim, dtype):
     out = check_attention(q, k, v, tables, positions)
     for _ in range(20):
         assert torch.equal(out, eb.paged_attention(q, k, v, tables, positions))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("vocab,spans", [
+    (50, [(5, 20)]), (50, [(0, 49)]), (1000, [(0, 1000)]), (1024, [(1, 1023)]),
+    (9000, [(3000, 5200)]), (9000, [(8192, 9000)]), (9000, [(0, 8192)]), (9000, [(2, 9000)]),
+    (20011, [(0, 16384)]), (20011, [(1, 20010)]), (30000, [(8000, 30000)])])
+def test_select_with_the_types_lowest_value_as_a_mask(vocab, spans, dtype):
+    """Spans, chunks and whole rows at the lowest finite value weigh nothing beside others, and are no dead beams."""
+    scores, ended = -torch.rand(2, 3).cumsum(1), torch.zeros(2, 3, dtype=torch.bool)
+    check_select(lowest_masked(dtype, vocab, spans), scores, ended, eos=-1)
+    check_select(lowest_masked(dtype, vocab, spans).neg(), scores, ended, eos=-1)
+
+
+@pytest.mark.parametrize("vocab", [300, 9000])
+def test_select_logits_far_from_zero(vocab):
+    """The log-probability is taken from the distance to the largest logit: no bits are lost to its size."""
+    logits = torch.randn(2, 3, vocab, generator=torch.Generator().manual_seed(1)) + 2.0 ** 16
+    check_select(logits, -torch.rand(2, 3).cumsum(1), torch.zeros(2, 3, dtype=torch.bool), eos=-1)
