@@ -4,7 +4,7 @@ import torch
 
 import exploration_b200 as eb
 from tests.test_decoding_edges import lowest_masked
-from tests.test_paged_gpu import check_attention, check_select, make_cache, queries, tail_positions
+from tests.test_paged_gpu import check_attention, check_select, make_cache, queries, select_inputs, tail_positions
 
 pytestmark = pytest.mark.gpu
 SIXTEEN = [torch.float16, torch.bfloat16]
@@ -47,3 +47,13 @@ def test_select_logits_far_from_zero(vocab):
     """The log-probability is taken from the distance to the largest logit: no bits are lost to its size."""
     logits = torch.randn(2, 3, vocab, generator=torch.Generator().manual_seed(1)) + 2.0 ** 16
     check_select(logits, -torch.rand(2, 3).cumsum(1), torch.zeros(2, 3, dtype=torch.bool), eos=-1)
+
+
+def test_select_many_beams_over_a_large_vocabulary():
+    """More chunk entries than the joining warp holds (32 beams x 13 chunks)."""
+    for beams in (20, 32):
+        check_select(*select_inputs(2, beams, 100003, torch.bfloat16, seed=beams), eos=2)
+    logits, scores, ended = select_inputs(1, 32, 100003, torch.float32)
+    logits[0, 3] = 1.5                       # ties over all chunks
+    logits[0, 4, 40:] = -float("inf")
+    check_select(logits, scores, ended, eos=2)
