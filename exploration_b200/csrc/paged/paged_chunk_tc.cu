@@ -21,14 +21,14 @@
 //
 // P (16 bit) overwrites its scores' TMEM columns; steps use the score buffers in
 // turn (three at head dim 64, two at 128), so with three a warpgroup finds its
-// next scores ready. A running maximum is kept until it grows by more than 2^8
-// (then O is rescaled in TMEM).
+// next scores ready. A row's reference point is kept until its maximum has grown past
+// it by more than 2^8 (2^4 in fp16); then O is rescaled in TMEM.
 //
 // TMEM columns: score buffers from 0, then the two accumulators of D columns.
 //
 // Measured: 2,048 tokens over 65,536 keys, 16 heads of 64, bf16: 0.64 ms in a short
 // burst (850 TFLOP/s), 0.76 ms sustained under the power cap (713); ragged chunks of
-// 1,111 tokens over up to 8,191 keys, 32/8 heads of 128, fp16: 0.355 and 0.41 ms (824).
+// 1,111 tokens over up to 8,191 keys, 32/8 heads of 128, fp16: 0.37 and 0.43 ms (780).
 // At head dim 64 a step is bound by the softmax instructions of two warps an SM
 // sub-partition (their special-function share alone is 2,048 cycles of 2,500) and the
 // hand-overs around them; at 128 by the chain weights -> P V -> next S -> softmax
@@ -65,7 +65,13 @@ constexpr int kTile = 128;            // keys of a tile
 constexpr int kBox = 128 * 64;        // elements of a 64-wide half of a 128-row operand
 constexpr int kThreads = 384;
 constexpr int kTmemCols = 512;
-constexpr float kRescale = 8.f;       // log2 units
+// How far a row's maximum may grow past its reference point before the accumulator is rescaled
+// (log2 units). In fp16 every unit of it is taken from the range of the weights (paged_mma.cuh): with 4
+// keys 2^-25 below the largest keep all bits, with 8 2^-21. Logits of standard deviation 2, ragged chunks
+// of 1,111 tokens over up to 8,191 keys, in a burst: 351 us with 8, 367 with 4, 385 with 2; 2,048
+// tokens over 32,768 keys, head dim 64: 328 us with 8, 347 with 4.
+template <typename T>
+constexpr float kRescale = std::is_same_v<T, __half> ? 4.f : 8.f;
 
 template <int D>
 struct alignas(1024) ChunkSmem {
@@ -376,6 +382,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     const int row = (warp & 3) * 32 + lane;          // TMEM lane
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t o_addr = lane_addr + kO + w * D;
+    constexpr float kBelow = std::is_same_v<T, __half> ? kWeightExp<T> - kRescale<T> : 0.f;
     int joins = 0;
     uint32_t done = 0;       // products this warpgroup has asked for
     uint32_t step0 = 0;      // steps of earlier items, both warpgroups'
@@ -441,13 +448,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           for (int i = 0; i < 4; ++i) top[i] = max3(top[i], x[c + i], x[c + 4 + i]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], x[kTile - 4 + i]);
-        const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+        const float peak = reference_point(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), p.scale_log2, kBelow);
         float alpha = 1.f;
-        if (peak > m + kRescale || m == kNegInf) {
-          alpha = ex2(m - finite_or_zero(peak));     // 0 at the first key
+        // A warp that has to rescale for one row takes the maxima of all its rows over.
+        const bool outgrown = __any_sync(0xffffffffu, peak > m + kRescale<T> || (m == kNegInf && peak > m));
+        if (outgrown && peak > m) {
+          alpha = ex2(m - peak);     // 0 at the first key
           m = peak;
         }
-        if (begun > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+        if (begun > 0 && outgrown) {
           if (!product_done()) {
             ok = false;
             break;

@@ -1,5 +1,5 @@
-// Warp-level matrix instructions of the few-row kernel, 16-bit packing and the
-// tcgen05 instruction descriptor of the chunk kernel.
+// Warp-level matrix instructions of the few-row kernel, 16-bit packing and range
+// of the weights, and the tcgen05 instruction descriptor of the chunk kernel.
 #pragma once
 
 #include <type_traits>
@@ -49,6 +49,18 @@ EB_DEVICE uint32_t pack2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
 }
+
+// Weights are rounded to the input type for the second product, and fp16 keeps 11 bits
+// down to 2^-14 only: relative to a largest weight of one, a key 2^-25 below it would
+// vanish, however many there are. Reference points therefore lie below the maximum so
+// that the largest weight is 2^kWeightExp; sums and partial results carry the same
+// factor, which cancels. bf16 has the range of fp32. Rounding a reference point
+// up keeps the largest weight from passing that power at logits beyond 2^24.
+template <typename T>
+constexpr float kWeightExp = std::is_same_v<T, __half> ? 15.f : 0.f;
+
+// Reference point of a row whose largest score is `top`, `below` the maximum (log2 units).
+EB_DEVICE float reference_point(float top, float scale_log2, float below) { return __fmaf_ru(top, scale_log2, -below); }
 
 // Bounded wait of the tile loops: sm100::mbar_wait without its sleep between
 // polls (the poll itself suspends the warp for a while); the time and the abort

@@ -237,7 +237,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           float t = fmaxf(fmaxf(a[0][2 * i], a[0][2 * i + 1]), fmaxf(a[1][2 * i], a[1][2 * i + 1]));
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-          const float next = fmaxf(m[i], t * p.scale_log2), ref = finite_or_zero(next);
+          const float next = fmaxf(m[i], reference_point(t, p.scale_log2, kWeightExp<T>)), ref = finite_or_zero(next);
           scale[i] = ex2(m[i] - ref);
           m[i] = next;
           float sum = 0.f;
@@ -260,7 +260,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             o[n][3] *= scale[1];
           }
         }
-        // Weights are rounded to the input type for the second product (their sum is not).
+        // Weights are rounded to the input type for the second product (their sum is not): at most
+        // 2^15 in fp16, so that keys 2^-29 below the largest keep their bits.
         const uint32_t w[4] = {pack2<T>(a[0][0], a[0][1]), pack2<T>(a[0][2], a[0][3]), pack2<T>(a[1][0], a[1][1]),
                                pack2<T>(a[1][2], a[1][3])};
         uint32_t keep[2] = {0xffffffffu, 0xffffffffu};

@@ -57,3 +57,24 @@ def test_select_many_beams_over_a_large_vocabulary():
     logits[0, 3] = 1.5                       # ties over all chunks
     logits[0, 4, 40:] = -float("inf")
     check_select(logits, scores, ended, eos=2)
+
+
+@pytest.mark.parametrize("dtype", SIXTEEN)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("gap", [4, 10, 14, 17, 19])
+@pytest.mark.parametrize("sink", [0, 700, 1499])
+@pytest.mark.parametrize("new,heads", [(1, 2), (5, 4), (40, 2), (300, 2)])
+def test_attention_one_key_takes_nearly_all_weight(new, heads, sink, gap, dim, dtype):
+    """A key of value zero ``gap`` (natural logarithm) above all others: the result is what the others hold."""
+    lengths = [1500 + new, 1800]
+    k, v, tables = make_cache(lengths, 2, dim, 64, dtype, seed=4)
+    k.mul_(0.05)
+    v.copy_(64 + 16 * v)                      # of one sign: a loss common to all weights does not average out
+    q = queries(2, new, heads, dim, dtype, scale=0.05)
+    q[..., 0] = 4.0
+    for b in range(2):
+        page, row = int(tables[b, sink // 64]), sink % 64
+        k[page, :, row] = 0
+        k[page, :, row, 0] = gap * dim ** 0.5 / 4
+        v[page, :, row] = 0
+    check_attention(q, k, v, tables, tail_positions(lengths, [new, new], new))
