@@ -57,6 +57,7 @@ beam_reorder_kernel(ReorderArgs p) {
   }
   if (!moves) return;
   const int from = theirs[tail];
+  // Also the end of a call on empty pools, which have no page.
   if (from < 0 || from >= p.pages || fresh < 0 || fresh >= p.pages) return;
   char* cache = (blockIdx.y & 1 ? p.v : p.k) + (blockIdx.y >> 1) * p.layer_bytes;
   const char* src = cache + from * p.page_bytes;
@@ -100,6 +101,7 @@ std::tuple<at::Tensor, at::Tensor> beam_reorder(at::Tensor& k_cache, at::Tensor&
                         lengths_in.dim() == 1 && lengths_in.size(0) == spare_in.size(0) && tables_in.size(2) >= 1,
                     "expected pools [layers, pages, kv_heads, page, head_dim], tables [groups, beams, width], "
                     "spare, parents [groups, beams] and lengths [groups]");
+  TORCH_CHECK_VALUE(k_cache.size(3) >= 1, "a page must hold at least one token");
   TORCH_CHECK_VALUE(k_cache.scalar_type() == v_cache.scalar_type() && k_cache.element_size() % 2 == 0,
                     "key and value pools must have one dtype of 16 bits or more");
   TORCH_CHECK_VALUE(tables_in.scalar_type() == at::kInt && spare_in.scalar_type() == at::kInt &&
@@ -130,13 +132,18 @@ std::tuple<at::Tensor, at::Tensor> beam_reorder(at::Tensor& k_cache, at::Tensor&
   args.row_bytes = row_bytes;
   args.head_bytes = args.page * row_bytes;
   args.page_bytes = args.kv_heads * args.head_bytes;
-  args.pages = k_cache.size(1);
+  // Pools without an element (no layers, heads, elements or pages) have nothing to copy: the tables alone are written.
+  const bool copies = k_cache.numel() > 0;
+  args.pages = copies ? k_cache.size(1) : 0;
   args.layer_bytes = args.pages * args.page_bytes;
   args.beams = spare.size(1);
   args.width = tables.size(2);
   // Heads of a CTA: about 16 KB of a full page, all of it in flight at once.
-  args.heads_per_cta = std::max<int64_t>(1, std::min<int64_t>(args.kv_heads, 16384 / args.head_bytes));
-  const dim3 grid(slots, std::max<int64_t>(1, 2 * layers), cdiv(args.kv_heads, args.heads_per_cta));
+  dim3 grid(slots);
+  if (copies) {
+    args.heads_per_cta = std::max<int64_t>(1, std::min<int64_t>(args.kv_heads, 16384 / args.head_bytes));
+    grid = dim3(slots, 2 * layers, cdiv(args.kv_heads, args.heads_per_cta));
+  }
   auto stream = at::cuda::getCurrentCUDAStream();
   const bool wide = row_bytes % 16 == 0 && reinterpret_cast<uintptr_t>(args.k) % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(args.v) % 16 == 0;

@@ -64,7 +64,8 @@ def beam_reorder(k_cache, v_cache, tables, spare, parents, lengths):
     group's beams. The first ``lengths % page`` rows of a parent's page being
     filled are copied into the spare page of each beam whose parent is another
     beam; that page takes its place in the new table and the old one becomes
-    the spare. The given tables are left as they are.
+    the spare. The given tables are left as they are. Pools without an element (no
+    layers, say) give the tables and copy nothing.
     """
     if k_cache.is_cuda:
         out = _native.native(k_cache).beam_reorder(k_cache, v_cache, tables, spare, parents, lengths)
@@ -74,6 +75,8 @@ def beam_reorder(k_cache, v_cache, tables, spare, parents, lengths):
             or parents.shape != spare.shape or lengths.shape != spare.shape[:1] or tables.shape[2] < 1:
         raise ValueError("expected pools [layers, pages, kv_heads, page, head_dim], tables [groups, beams, width], "
                          "spare, parents [groups, beams] and lengths [groups]")
+    if k_cache.shape[3] < 1:
+        raise ValueError("a page must hold at least one token")
     if k_cache.dtype != v_cache.dtype or k_cache.dtype.itemsize % 2:
         raise ValueError("key and value pools must have one dtype of 16 bits or more")
     if tables.dtype != torch.int32 or spare.dtype != torch.int32 or lengths.dtype != torch.int32 \

@@ -96,3 +96,29 @@ def test_select_with_the_types_lowest_value_as_a_mask(dtype):
         want = select_reference(logits.double(), scores, ended, -1)
         torch.testing.assert_close(got[0], want[0], atol=2e-5, rtol=0)
         assert all(torch.equal(a, b) for a, b in zip(got[1:], want[1:]))
+
+
+EMPTY_POOLS = [(0, 12, 2, 16, 8), (2, 12, 0, 16, 8), (2, 12, 2, 16, 0)]     # no layers, no heads, no elements
+
+
+def reorder_inputs(shape, device="cpu"):
+    """Pools of ``shape`` and three beams, 21 tokens each, of which two take over the second one's state."""
+    k, v = torch.zeros(shape, device=device), torch.zeros(shape, device=device)
+    tables = torch.arange(9, dtype=torch.int32, device=device).view(1, 3, 3)
+    spare = torch.arange(9, 12, dtype=torch.int32, device=device).view(1, 3)
+    return k, v, tables, spare, torch.tensor([[1, 1, 1]], device=device), \
+        torch.tensor([21], dtype=torch.int32, device=device)
+
+
+REORDERED = [[[3, 9, 2], [3, 4, 5], [3, 11, 8]]], [[1, 10, 7]]
+
+
+@pytest.mark.parametrize("shape", EMPTY_POOLS)
+def test_reorder_of_empty_pools(shape):
+    fresh, freed = eb.beam_reorder(*reorder_inputs(shape))
+    assert (fresh.tolist(), freed.tolist()) == REORDERED
+
+
+def test_reorder_refuses_pages_without_tokens():
+    with pytest.raises(ValueError, match="at least one token"):
+        eb.beam_reorder(*reorder_inputs((2, 12, 2, 0, 8)))

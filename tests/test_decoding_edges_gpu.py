@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import exploration_b200 as eb
-from tests.test_decoding_edges import lowest_masked
+from tests.test_decoding_edges import EMPTY_POOLS, REORDERED, lowest_masked, reorder_inputs
 from tests.test_paged_gpu import check_attention, check_select, make_cache, queries, select_inputs, tail_positions
 
 pytestmark = pytest.mark.gpu
@@ -78,3 +78,14 @@ def test_attention_one_key_takes_nearly_all_weight(new, heads, sink, gap, dim, d
         k[page, :, row, 0] = gap * dim ** 0.5 / 4
         v[page, :, row] = 0
     check_attention(q, k, v, tables, tail_positions(lengths, [new, new], new))
+
+
+@pytest.mark.parametrize("shape", EMPTY_POOLS + [(2, 12, 2, 16, 8)])
+def test_reorder_of_empty_pools(shape):
+    fresh, freed = eb.beam_reorder(*reorder_inputs(shape, "cuda"))
+    assert (fresh.tolist(), freed.tolist()) == REORDERED
+
+
+def test_reorder_refuses_pages_without_tokens():
+    with pytest.raises(ValueError, match="at least one token"):
+        eb.beam_reorder(*reorder_inputs((2, 12, 2, 0, 8), "cuda"))
