@@ -85,7 +85,7 @@ struct alignas(1024) ChunkSmem {
   uint16_t v[kStages][kTile * D];
   uint64_t q_full, q_empty;
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[kBufs], p_full[kBufs], p_half[kBufs], join, v_ragged, v_clear;
+  uint64_t s_full[kBufs], p_full[kBufs], p_half[kBufs], join, v_ragged, v_clear, drained;
   uint64_t o_done[2][kProductBarriers];   // of each warpgroup, its products in turn (paged_phases.h)
   uint32_t tmem_base;
   int abort;
@@ -178,6 +178,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     mbar_init(&sm.join, 256);
     mbar_init(&sm.v_ragged, 1);
     mbar_init(&sm.v_clear, 1);
+    mbar_init(&sm.drained, 1);
     sm.abort = 0;
     fence_barrier_init();
   }
@@ -206,8 +207,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       prefetch_tensormap(&tk);
       prefetch_tensormap(&tv);
     }
-    Ring ring;            // K and V advance together
-    int q_loads = 0, tiles_issued = 0;
+    CopyRing k_ring, v_ring;
+    int q_loads = 0;
     bool ok = true;
     while (ok && walk.next(p, sm.table, s)) {
       // The first entries are on their way before the limit is known (the table has them all).
@@ -247,12 +248,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         const int plane = id >= 0 && id < p.pages ? id * p.kv_heads + kv_head : p.pages * p.kv_heads;
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-          uint64_t* full = part == 0 ? &sm.k_full[ring.stage] : &sm.v_full[ring.stage];
-          uint64_t* empty = part == 0 ? &sm.k_empty[ring.stage] : &sm.v_empty[ring.stage];
-          uint16_t* dst = part == 0 ? sm.k[ring.stage] : sm.v[ring.stage];
+          CopyRing& ring = part == 0 ? k_ring : v_ring;
+          const Phase slot = ring.next(kStages);
+          uint64_t* full = part == 0 ? &sm.k_full[slot.barrier] : &sm.v_full[slot.barrier];
+          uint64_t* empty = part == 0 ? &sm.k_empty[slot.barrier] : &sm.v_empty[slot.barrier];
+          uint16_t* dst = part == 0 ? sm.k[slot.barrier] : sm.v[slot.barrier];
           const CUtensorMap* map = part == 0 ? &tk : &tv;
-          if (tiles_issued >= kStages &&
-              !__all_sync(0xffffffffu, wait_tight(empty, ring.phase ^ 1, abort, err, kSiteKvEmpty))) {
+          if (ring.reuses(kStages) &&
+              !__all_sync(0xffffffffu, wait_tight(empty, slot.parity ^ 1, abort, err, kSiteKvEmpty))) {
             ok = false;
             break;
           }
@@ -264,17 +267,18 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
               tma_load_3d(dst + h * kBox + lane * box * 64, map, full, h * 64, (key0 + lane * box) & (p.page - 1),
                           plane);
           }
+          ++ring.issued;
         }
         if (!ok) break;
-        ++tiles_issued;
-        ring.next(kStages);
       }
     }
     if (*abort && lane == 0) {   // let issued copies land before the CTA exits
-      for (int j = max(0, tiles_issued - kStages); j < tiles_issued; ++j) {
-        mbar_wait(&sm.k_full[j % kStages], (j / kStages) & 1, abort, nullptr, kSiteDrain);
-        mbar_wait(&sm.v_full[j % kStages], (j / kStages) & 1, abort, nullptr, kSiteDrain);
-      }
+      k_ring.drain(kStages, [&](uint32_t stage, uint32_t parity) {
+        mbar_wait(&sm.k_full[stage], parity, abort, nullptr, kSiteDrain);
+      });
+      v_ring.drain(kStages, [&](uint32_t stage, uint32_t parity) {
+        mbar_wait(&sm.v_full[stage], parity, abort, nullptr, kSiteDrain);
+      });
       if (q_loads > 0) mbar_wait(&sm.q_full, (q_loads - 1) & 1, abort, nullptr, kSiteDrain);
     }
   } else if (warp == 1) {
@@ -355,6 +359,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         }
       }
       ok = __all_sync(0xffffffffu, ok);
+    }
+    if (*abort && elect_one()) {   // issued products read shared memory and TMEM: let them end first
+      tc_commit(&sm.drained);
+      mbar_wait(&sm.drained, 0, abort, nullptr, kSiteDrain);
     }
   } else if (warp == 3) {
     // Rows past an item's limit in its last value tile: cleared when warp 1 has seen the tile arrive.

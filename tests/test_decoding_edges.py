@@ -122,3 +122,45 @@ def test_reorder_of_empty_pools(shape):
 def test_reorder_refuses_pages_without_tokens():
     with pytest.raises(ValueError, match="at least one token"):
         eb.beam_reorder(*reorder_inputs((2, 12, 2, 0, 8)))
+
+
+# Keys and values go out in turn, tile by tile; a producer that gives up after any number of copies waits
+# for all that may be under way: the newest `stages` of each operand, each wait passing only once that copy
+# has landed (the one before it in its slot has, or the slot would not have been reused).
+COPIES = r"""
+#include <cstdio>
+#include "paged_phases.h"
+using namespace eb::paged;
+
+int main() {
+  long long wrong = 0, cases = 0;
+  for (uint32_t stages = 2; stages <= 4; stages += 2)
+    for (uint32_t copies = 0; copies < 40; ++copies) {
+      CopyRing rings[2];
+      for (uint32_t i = 0; i < copies; ++i) {
+        CopyRing& ring = rings[i & 1];
+        const Phase slot = ring.next(stages);
+        wrong += slot.barrier != ring.issued % stages || ring.reuses(stages) != (ring.issued >= stages);
+        ++ring.issued;
+      }
+      for (int part = 0; part < 2; ++part) {
+        const uint32_t issued = (copies + 1 - part) / 2;
+        wrong += rings[part].issued != issued;
+        uint32_t n = issued > stages ? issued - stages : 0;
+        rings[part].drain(stages, [&](uint32_t slot, uint32_t parity) {
+          const uint32_t before = n / stages;        // phases of the slot's barrier without copy n
+          wrong += slot != n % stages || (before & 1) != parity || ((before + 1) & 1) == parity;
+          ++n;
+          ++cases;
+        });
+        wrong += n != issued;
+      }
+    }
+  std::printf("%lld %lld\n", wrong, cases);
+}
+"""
+
+
+def test_a_producer_that_gives_up_waits_for_every_copy(tmp_path):
+    wrong, waits = run_host_program(tmp_path, COPIES)
+    assert wrong == 0 and waits > 100
