@@ -4,17 +4,28 @@ The prompt is encoded in chunks (:func:`paged_append`, :func:`paged_attention`
 in every layer), then every step runs one token a beam, takes the best
 continuations (:func:`beam_select`) and lets the cache follow them
 (:func:`beam_reorder`). Lengths, positions, tables and the selection stay on
-the device; the host looks at them only to stop early.
+the device; the host looks at them only to stop early, and at the end for
+kernels that gave up a wait.
 """
 from __future__ import annotations
 
 import torch
 
-from ..ops import fused
+from ..ops import _native, fused
 from ..ops.beam import MAX_BEAMS, beam_reorder, beam_select
 from ..ops.paged import MIN_PAGE
 
 STOP_EVERY = 16      # steps between looks at whether every beam has ended
+
+
+def check_waits(device):
+    """Raises when a kernel on ``device`` gave up a bounded wait: what it should have written is undefined."""
+    if device.type != "cuda":
+        return
+    torch.cuda.current_stream(device).synchronize()
+    site, cta = _native.load().device_errors(device.index)
+    if site:
+        raise RuntimeError(f"a kernel on {device} gave up a wait (site {site}, CTA {cta}): its results are undefined")
 
 
 class PagedCache:
@@ -77,7 +88,8 @@ def generate(model, prompts, max_new_tokens, *, beams=1, eos=None, page=64, pref
     ``prompts`` is a list of token lists (or 1-D tensors) of any lengths;
     ``beams=1`` is greedy decoding. ``scores`` are cumulative log-probabilities,
     best first; a hypothesis that ended is padded with ``eos``. ``n`` is at most
-    ``max_new_tokens`` (less when every beam has ended).
+    ``max_new_tokens`` (less when every beam has ended). On a GPU the call waits
+    for its result and raises ``RuntimeError`` when a kernel gave up a wait.
     """
     _check(model, prompts, max_new_tokens, beams, eos, prefill_chunk)
     device = model.embedding.weight.device
@@ -123,11 +135,13 @@ def generate(model, prompts, max_new_tokens, *, beams=1, eos=None, page=64, pref
         if step + 1 == max_new_tokens:
             break
         if eos is not None and step % STOP_EVERY == STOP_EVERY - 1 and bool(finished.all()):
-            return out[:, :, :step + 1], scores
+            out = out[:, :, :step + 1]
+            break
         if beams > 1:
             cache.reorder(parents)
         at = cache.lengths[:, None].expand(groups, beams).reshape(-1, 1)
         x = run(tokens.reshape(-1, 1), at, cache.rows)
         cache.lengths += 1
         logits = model.logits(x).view(groups, beams, -1)
+    check_waits(device)
     return out, scores

@@ -1,4 +1,5 @@
 """Decoding operators and generation at their edges: what can be checked without a GPU."""
+import importlib
 import shutil
 import subprocess
 from pathlib import Path
@@ -164,3 +165,34 @@ int main() {
 def test_a_producer_that_gives_up_waits_for_every_copy(tmp_path):
     wrong, waits = run_host_program(tmp_path, COPIES)
     assert wrong == 0 and waits > 100
+
+
+def test_generate_raises_when_a_kernel_gave_up_a_wait(monkeypatch):
+    generation = importlib.import_module("exploration_b200.runtime.generate")
+    torch.manual_seed(0)
+    model, looked = eb.BaselineModel(19, dim=32, heads=4, layers=1).eval(), []
+    monkeypatch.setattr(generation, "check_waits", looked.append)
+    eb.generate(model, [[1, 2], [3]], 3, page=16)
+    assert looked == [torch.device("cpu")]
+    monkeypatch.undo()
+
+    # The error word of a device, read and cleared: (site, CTA).
+    words = {1: [(2, 37), (0, 0)]}
+    order = []
+
+    class Extension:
+        def device_errors(self, index):
+            order.append("read")
+            return words[index].pop(0)
+
+    class Stream:
+        def synchronize(self):
+            order.append("synchronize")
+
+    monkeypatch.setattr(generation._native, "load", lambda: Extension())
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: Stream())
+    with pytest.raises(RuntimeError, match="site 2, CTA 37"):
+        generation.check_waits(torch.device("cuda", 1))
+    generation.check_waits(torch.device("cuda", 1))
+    generation.check_waits(torch.device("cpu"))
+    assert order == ["synchronize", "read"] * 2
