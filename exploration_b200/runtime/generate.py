@@ -104,6 +104,8 @@ def generate(model, prompts, max_new_tokens, *, beams=1, eos=None, page=64, pref
     for g, p in enumerate(prompts):
         ids[g, :len(p)] = p
         positions[g, :len(p)] = torch.arange(len(p), dtype=torch.int32)
+    if bool(((ids < 0) | (ids >= model.embedding.weight.shape[0])).any()):
+        raise ValueError("prompt tokens must lie in the model's vocabulary")     # on a GPU a fault of its embedding
     ids, positions = ids.to(device), positions.to(device)
     cos, sin = model.rope.tables(torch.arange(longest + max_new_tokens, device=device))
 

@@ -196,3 +196,12 @@ def test_generate_raises_when_a_kernel_gave_up_a_wait(monkeypatch):
     generation.check_waits(torch.device("cuda", 1))
     generation.check_waits(torch.device("cpu"))
     assert order == ["synchronize", "read"] * 2
+
+
+@pytest.mark.parametrize("prompt", [[1, 19], [-1], torch.tensor([3, 400])])
+def test_generate_refuses_tokens_outside_the_vocabulary(prompt):
+    torch.manual_seed(0)
+    model = eb.BaselineModel(19, dim=32, heads=4, layers=1).eval()
+    eb.generate(model, [[0, 18]], 1, page=16)
+    with pytest.raises(ValueError, match="vocabulary"):
+        eb.generate(model, [[1], prompt], 1, page=16)
