@@ -110,6 +110,7 @@ std::tuple<at::Tensor, at::Tensor> beam_reorder(at::Tensor& k_cache, at::Tensor&
   TORCH_CHECK_VALUE(same_device(k_cache, v_cache, tables_in, spare_in, parents_in, lengths_in),
                     "all tensors must be on one device");
   TORCH_CHECK_VALUE(k_cache.is_contiguous() && v_cache.is_contiguous(), "cache pools must be contiguous");
+  TORCH_CHECK_VALUE(!wants_grad(k_cache) && !wants_grad(v_cache), "beam_reorder is for inference: it has no gradient");
   c10::cuda::CUDAGuard guard(k_cache.device());
   const at::Tensor tables = tables_in.contiguous(), spare = spare_in.contiguous(), parents = parents_in.contiguous(),
                    lengths = lengths_in.contiguous();

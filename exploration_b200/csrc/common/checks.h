@@ -6,7 +6,10 @@
 
 namespace eb {
 
-inline bool wants_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+// A gradient would have to flow through `t`: backward, or forward as a dual number's tangent.
+inline bool wants_grad(const at::Tensor& t) {
+  return (at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(/*level=*/0).defined();
+}
 
 template <typename... Rest>
 bool same_device(const at::Tensor& first, const Rest&... rest) {

@@ -128,7 +128,8 @@ at::Tensor paged_append(const at::Tensor& q_in, const at::Tensor& k_in, const at
   TORCH_CHECK_VALUE(cos_in.sizes() == sin_in.sizes() && cos_in.dim() == 2 && cos_in.size(1) * 2 == q_in.size(3) &&
                         cos_in.scalar_type() == at::kFloat && sin_in.scalar_type() == at::kFloat,
                     "expected fp32 cos, sin [positions, head_dim / 2]");
-  TORCH_CHECK_VALUE(!wants_grad(k_in) && !wants_grad(v_in), "paged operators are for inference: they have no gradient");
+  TORCH_CHECK_VALUE(!wants_grad(k_in) && !wants_grad(v_in) && !wants_grad(cos_in) && !wants_grad(sin_in),
+                    "paged operators are for inference: they have no gradient");
   c10::cuda::CUDAGuard guard(q_in.device());
   auto rows = [](const at::Tensor& t) { return t.stride(3) == 1 ? t : t.contiguous(); };
   const at::Tensor q = rows(q_in), k = rows(k_in), v = rows(v_in), cos = cos_in.contiguous(), sin = sin_in.contiguous();

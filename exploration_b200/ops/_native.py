@@ -13,6 +13,7 @@ import importlib.util
 from pathlib import Path
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 EXT_NAME = "eb200_C"
 BUILD_DIR = Path(__file__).resolve().parents[1] / "_build"
@@ -56,6 +57,13 @@ def load(required: bool = True):
 
 def available() -> bool:
     return load(required=False) is not None
+
+
+def wants_grad(*tensors) -> bool:
+    """Whether a gradient would have to flow through one of ``tensors``, backward or as a tangent."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        return True
+    return any(t.is_floating_point() and unpack_dual(t).tangent is not None for t in tensors)
 
 
 def native(tensor: torch.Tensor):

@@ -47,7 +47,7 @@ def beam_select(logits, scores, finished, eos):
         raise ValueError("all tensors must be on one device")
     if not 1 <= logits.shape[1] <= MAX_BEAMS or logits.shape[2] < 1:
         raise ValueError(f"between 1 and {MAX_BEAMS} beams and at least one token")
-    if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
+    if _native.wants_grad(logits, scores):
         raise ValueError("beam_select is for inference: it has no gradient")
     eos = int(eos)
     if not -1 <= eos < logits.shape[2]:
@@ -86,6 +86,8 @@ def beam_reorder(k_cache, v_cache, tables, spare, parents, lengths):
         raise ValueError("all tensors must be on one device")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("cache pools must be contiguous")
+    if _native.wants_grad(k_cache, v_cache):
+        raise ValueError("beam_reorder is for inference: it has no gradient")
     return reorder_reference(k_cache, v_cache, tables, spare, parents, lengths)
 
 

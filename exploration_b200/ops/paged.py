@@ -60,7 +60,7 @@ def _check_cache(x, k_cache, v_cache, tables, positions):
     device = x.device
     if not (k_cache.device == v_cache.device == tables.device == positions.device == device):
         raise ValueError("all tensors must be on one device")
-    if torch.is_grad_enabled() and (x.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+    if _native.wants_grad(x, k_cache, v_cache):
         raise ValueError("paged operators are for inference: they have no gradient")
 
 
@@ -84,7 +84,7 @@ def paged_append(q, k, v, cos, sin, k_cache, v_cache, tables, positions):
     if cos.shape != sin.shape or cos.ndim != 2 or cos.shape[1] * 2 != q.shape[3] \
             or cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise ValueError("expected fp32 cos, sin [positions, head_dim / 2]")
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+    if _native.wants_grad(k, v, cos, sin):
         raise ValueError("paged operators are for inference: they have no gradient")
     return append_reference(q, k, v, cos, sin, k_cache, v_cache, tables, positions)
 

@@ -205,3 +205,43 @@ def test_generate_refuses_tokens_outside_the_vocabulary(prompt):
     eb.generate(model, [[0, 18]], 1, page=16)
     with pytest.raises(ValueError, match="vocabulary"):
         eb.generate(model, [[1], prompt], 1, page=16)
+
+
+def decoding_calls(device="cpu"):
+    """Every decoding operator with the names of its differentiable inputs."""
+    def new(*shape):
+        return torch.randn(*shape, device=device)
+
+    tables, positions = (torch.zeros(1, n, dtype=torch.int32, device=device) for n in (1, 2))
+    paged = {"q": new(1, 2, 4, 8), "k": new(1, 2, 2, 8), "v": new(1, 2, 2, 8), "cos": new(20, 4), "sin": new(20, 4),
+             "k_cache": new(3, 2, 16, 8), "v_cache": new(3, 2, 16, 8)}
+    attention = {n: paged[n].clone() for n in ("q", "k_cache", "v_cache")}
+    select = {"logits": new(2, 3, 5), "scores": new(2, 3)}
+    ended = torch.zeros(2, 3, dtype=torch.bool, device=device)
+    k, v, *rest = reorder_inputs((2, 12, 2, 16, 8), device)
+    return [
+        (lambda **x: eb.paged_append(*x.values(), tables, positions), paged),
+        (lambda **x: eb.paged_attention(*x.values(), tables, positions), attention),
+        (lambda **x: eb.beam_select(*x.values(), ended, 1), select),
+        (lambda **x: eb.beam_reorder(*x.values(), *rest), {"k_cache": k, "v_cache": v}),
+    ]
+
+
+def check_gradients_are_refused(device):
+    from torch.autograd import forward_ad
+    for call, inputs in decoding_calls(device):
+        call(**inputs)
+        for name, x in inputs.items():
+            leaf = x.clone().requires_grad_()
+            with pytest.raises(ValueError, match="no gradient"):
+                call(**{**inputs, name: leaf})
+            with torch.no_grad():
+                call(**{**inputs, name: leaf})
+                with forward_ad.dual_level():
+                    with pytest.raises(ValueError, match="no gradient"):
+                        call(**{**inputs, name: forward_ad.make_dual(x.clone(), torch.ones_like(x))})
+                    call(**inputs)
+
+
+def test_gradients_and_tangents_are_refused():
+    check_gradients_are_refused("cpu")

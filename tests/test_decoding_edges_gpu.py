@@ -3,7 +3,8 @@ import pytest
 import torch
 
 import exploration_b200 as eb
-from tests.test_decoding_edges import EMPTY_POOLS, REORDERED, lowest_masked, reorder_inputs
+from tests.test_decoding_edges import (EMPTY_POOLS, REORDERED, check_gradients_are_refused, lowest_masked,
+                                       reorder_inputs)
 from tests.test_paged_gpu import check_attention, check_select, make_cache, queries, select_inputs, tail_positions
 
 pytestmark = pytest.mark.gpu
@@ -89,3 +90,7 @@ def test_reorder_of_empty_pools(shape):
 def test_reorder_refuses_pages_without_tokens():
     with pytest.raises(ValueError, match="at least one token"):
         eb.beam_reorder(*reorder_inputs((2, 12, 2, 0, 8), "cuda"))
+
+
+def test_gradients_and_tangents_are_refused():
+    check_gradients_are_refused("cuda")
