@@ -94,3 +94,15 @@ def test_reorder_refuses_pages_without_tokens():
 
 def test_gradients_and_tangents_are_refused():
     check_gradients_are_refused("cuda")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("batch,new,dim", [(1030, 20, 64), (530, 300, 64), (1030, 20, 128)])
+def test_attention_chunks_of_many_sequences(batch, new, dim, dtype):
+    """More row tiles than the split's table holds: one item a CTA in the chunk kernel and the fp32 tiles."""
+    lengths = [1 + (i * 53) % 450 for i in range(batch)]
+    k, v, tables = make_cache(lengths, 1, dim, 32, dtype)
+    positions = tail_positions(lengths, [min(n, new) for n in lengths], new)
+    positions[11] = -1
+    out = check_attention(queries(batch, new, 2, dim, dtype), k, v, tables, positions)
+    assert not out[11].any()
