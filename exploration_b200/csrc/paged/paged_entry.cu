@@ -24,7 +24,8 @@ enum class Path { kCudaCore, kTileFp32, kRows, kChunk };
 Path choose(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache) {
   const int64_t dim = q.size(3);
   auto aligned = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; };
-  if ((dim != 64 && dim != 128) || !aligned(q) || !aligned(k_cache) || !aligned(v_cache)) return Path::kCudaCore;
+  const bool q_aligned = !q.is_contiguous() || aligned(q);   // strided queries are copied first
+  if ((dim != 64 && dim != 128) || !q_aligned || !aligned(k_cache) || !aligned(v_cache)) return Path::kCudaCore;
   const int64_t rows = q.size(1) * (q.size(2) / k_cache.size(1));
   if (q.scalar_type() == at::kFloat) return rows <= 4 ? Path::kCudaCore : Path::kTileFp32;
   return rows <= 16 ? Path::kRows : Path::kChunk;

@@ -106,3 +106,18 @@ def test_attention_chunks_of_many_sequences(batch, new, dim, dtype):
     positions[11] = -1
     out = check_attention(queries(batch, new, 2, dim, dtype), k, v, tables, positions)
     assert not out[11].any()
+
+
+def test_attention_record_names_the_kernel_that_ran():
+    """Queries that are copied before the call are aligned, wherever the view began."""
+    from exploration_b200.ops import launch
+    k, v, tables = make_cache([90], 2, 64, 16, torch.bfloat16)
+    base = torch.randn(2 * (1 * 40 * 8 * 64) + 1, device="cuda").to(torch.bfloat16)
+    wide = base[1:].view(1, 40, 8, 128)[..., :64]
+    assert wide.data_ptr() % 16 and not wide.is_contiguous()
+    launch.reset()
+    positions = tail_positions([90], [40], 40)
+    out = eb.paged_attention(wide, k, v, tables, positions)
+    assert torch.equal(out, eb.paged_attention(wide.contiguous(), k, v, tables, positions))
+    [entry] = [e for e in launch.launch_report() if e["kernel"] == "paged_attention"]
+    assert entry["calls"] == 2 and entry["path"] == "tcgen05"
