@@ -121,3 +121,51 @@ def test_attention_record_names_the_kernel_that_ran():
     assert torch.equal(out, eb.paged_attention(wide.contiguous(), k, v, tables, positions))
     [entry] = [e for e in launch.launch_report() if e["kernel"] == "paged_attention"]
     assert entry["calls"] == 2 and entry["path"] == "tcgen05"
+
+
+@pytest.mark.parametrize("vocab", [50, 9000])
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_whole_step_can_be_captured(new, vocab):
+    """Append, attention, selection and reordering in one graph, replayed at other lengths."""
+    torch.manual_seed(0)
+    layers, groups, beams, heads, dim, page, width = 2, 2, 3, 4, 64, 16, 100
+    pages = groups * beams * (width + 1)
+    k, v = (torch.randn(layers, pages, heads, page, dim, device="cuda").to(torch.bfloat16) for _ in range(2))
+    order = torch.randperm(pages, device="cuda").to(torch.int32).view(groups, beams, width + 1)
+    tables, spare = order[..., :width].contiguous(), order[..., width].contiguous()
+    qkv = torch.randn(layers, groups * beams, new, 3, heads, dim, device="cuda").to(torch.bfloat16)
+    cos, sin = torch.rand(width * page, dim // 2, device="cuda"), torch.rand(width * page, dim // 2, device="cuda")
+    logits, scores = torch.randn(groups, beams, vocab, device="cuda"), -torch.rand(groups, beams, device="cuda")
+    ended = torch.zeros(groups, beams, dtype=torch.bool, device="cuda")
+    lengths = torch.tensor([1200, 700], dtype=torch.int32, device="cuda")
+
+    def step():
+        last = lengths[:, None].expand(groups, beams).reshape(-1, 1)
+        positions = last + torch.arange(new, device="cuda", dtype=torch.int32)
+        outs = []
+        for i in range(layers):
+            q = eb.paged_append(*qkv[i].unbind(2), cos, sin, k[i], v[i], tables.flatten(0, 1), positions)
+            outs.append(eb.paged_attention(q, k[i], v[i], tables.flatten(0, 1), positions))
+        picked = eb.beam_select(logits, scores, ended, 3)
+        moved = eb.beam_reorder(k, v, tables, spare, picked[1], lengths + new)
+        return [*outs, *picked, *moved]
+
+    start = k.clone(), v.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for n in ([1200, 700], [16, 1], [1500, 1499]):
+        lengths.copy_(torch.tensor(n, dtype=torch.int32))
+        logits.normal_()
+        results = []
+        for run in (graph.replay, step):
+            k.copy_(start[0])
+            v.copy_(start[1])
+            got = run()
+            results.append([x.clone() for x in (got or captured)] + [k.clone(), v.clone()])
+        assert all(torch.equal(a, b) for a, b in zip(*results))
