@@ -160,13 +160,14 @@ void paged_combine_launch(const Args& args, int ctas, cudaStream_t stream) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attr;
   config.numAttrs = 1;
-  // The many-row form reads 16-byte vectors: more than 16 rows come from the
-  // tensor-core kernel only, whose head dims allow them.
+  // The many-row form reads 16-byte vectors: more than 16 rows of an item come from the chunk
+  // kernel and the fp32 tiles only, whose head dims are 64 and 128.
   if (rows <= 16) {
     config.gridDim = dim3(ctas - 1, rows);
     config.blockDim = dim3(128);
     EB_CUDA_CHECK(cudaLaunchKernelEx(&config, paged_combine_row_kernel<T>, args));
   } else {
+    TORCH_CHECK(args.dim % 4 == 0, "paged_attention: many-row items need head dims of whole vectors");
     config.gridDim = dim3(ctas - 1, std::min(16, cdiv(rows * args.dim / 4, 256)));
     config.blockDim = dim3(256);
     EB_CUDA_CHECK(cudaLaunchKernelEx(&config, paged_combine_rows_kernel<T>, args));

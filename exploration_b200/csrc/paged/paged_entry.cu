@@ -17,10 +17,15 @@ enum class Path { kCudaCore, kTileFp32, kRows, kChunk };
 
 // The kernel of a call. Head dims 64 and 128 (one or two 128-byte swizzle spans of
 // a 16-bit type) have kernels of their own: up to 16 rows of a key head are bound
-// by the read of the cache, more by arithmetic. fp32 takes the general kernel for
-// up to four rows and the tiled one for more (four sequences over 30,000 keys, 16
-// heads of 64: 4 tokens 302 us in the general kernel; 12 tokens 941 us there, 364 us
-// in tiles).
+// by the read of the cache, more by arithmetic. Measured with four sequences over
+// 30,000 keys, 16 heads of 64:
+//   bf16, few-row / chunk kernel: 8 rows 86 / 98 us, 16 rows 90 / 100, 17 rows 157
+//     (keys read twice) / 99; over 500 keys 16 rows 14 / 21;
+//   fp32, general / tiled kernel: 2 rows 219 / 363 us, 4 rows 304 / 363, 5 rows
+//     352 / 364, 6 rows 402 / 363, 12 rows 941 / 365.
+// Five rows are a tie; 8 key heads of 128 give 233 / 399 us for 2 rows and 381 / 396 for 5.
+// Over a few hundred keys the tiles win from fewer rows on (4 rows of 8 key heads of
+// 128 over 500 keys: 41 / 20 us), which the rule does not use: the host does not know lengths.
 Path choose(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache) {
   const int64_t dim = q.size(3);
   auto aligned = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; };

